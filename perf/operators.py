@@ -187,8 +187,13 @@ def _own_context():
 
 
 def _run_own(s):
+    ctx = _own_context()
+    with torch.cuda.stream(ctx.stream):  # as a program that works on the framework's stream
+        return _calls(ctx, s["case"], s)
+
+
+def _calls(ctx, c, s):
     from flux2mi.api import MXFP4
-    c, ctx = s["case"], _own_context()
     if c["op"] == "quantize":
         q = ctx.op_quantize_mxfp4(s["x"])
         return {"values": ctx.op_dequantize_mxfp4(q, dtype=s["x"].dtype), "scales": q.scales}
