@@ -47,6 +47,18 @@ class StepContext(C.Structure):
                 ("sigma_next", C.c_float), ("height", C.c_int), ("width", C.c_int), ("is_i2i", C.c_int)]
 
 
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class ResidualNorm(C.Structure):
+    _fields_ = [("rows", C.c_int), ("dim", C.c_int), ("split", C.c_int), ("post_norm", C.c_int), ("norm", C.c_int),
+                ("post_eps", C.c_float), ("eps", C.c_float), ("resid_scale", C.c_float),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p), ("y_dtype", C.c_int), ("ldy", C.c_int64),
+                ("x_out", C.c_void_p), ("ldx_out", C.c_int64), ("out", C.c_void_p), ("out_dtype", C.c_int), ("ldo", C.c_int64),
+                ("post_weight", C.c_void_p), ("weight", C.c_void_p),
+                ("gate", C.c_void_p * 2), ("scale", C.c_void_p * 2), ("shift", C.c_void_p * 2)]
+
+
 STEP_HOOK = C.CFUNCTYPE(C.c_int, C.POINTER(StepContext), C.c_void_p, C.c_void_p, C.c_void_p)
 PROGRESS_CB = C.CFUNCTYPE(None, C.c_int, C.c_int, C.c_void_p)
 CHECKPOINT_CB = C.CFUNCTYPE(None, C.c_int, C.POINTER(C.c_uint8), C.c_int, C.c_int, C.c_void_p)
@@ -206,6 +218,13 @@ PROTOTYPES = {
     "flux2mi_op_attention_prescaled": (_I, [_P, _P, _P, _I, _I, C.c_float]),
     "flux2mi_op_attention_qk8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, C.c_float]),
     "flux2mi_op_attention_prescaled_range": (_I, [_P, _P, _P, _I, _I, C.c_float, _I, _I, _I]),
+    "flux2mi_mxfp4_code_bytes": (_I64, [_I64, _I64]),
+    "flux2mi_mxfp4_scale_bytes": (_I64, [_I64, _I64]),
+    "flux2mi_op_quantize_mxfp4": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P]),
+    "flux2mi_op_dequantize_mxfp4": (_I, [_P, _P, _P, _I64, _I64, _P, _I, _I64]),
+    "flux2mi_op_gemm_mxfp4": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I, _I64, _I, _I, _I]),
+    "flux2mi_op_gemm_bf16_mxfp4": (_I, [_P, _P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I, _I64, _I, _I, _I]),
+    "flux2mi_op_residual_norm": (_I, [_P, C.POINTER(ResidualNorm)]),
 }
 
 _lib = None

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import weakref
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -87,6 +87,18 @@ def _req(t: torch.Tensor, dtype, name: str) -> torch.Tensor:
     return t.contiguous()
 
 
+class MXFP4(NamedTuple):
+    """A matrix [rows, cols] in microscaled 4-bit floating point (include/flux2mi.h, "MXFP4"): 32 values of a row share one power of two.
+    codes u8 [rows, P / 2] and scales u8 [rows, P / 32], P = cols rounded up to a multiple of 128, the padding zero."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    cols: int
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+
 class Context:
     """One GPU + one HIP stream + one generation in flight (flux2mi_ctx)."""
 
@@ -101,12 +113,16 @@ class Context:
         self.handle = h
         self._children = []  # weakrefs of DiT / VAE objects: they must be destroyed before the context
 
-    # stream ordering against torch's current stream (no host sync)
+    # stream ordering against torch's current stream (no host sync; nothing to order inside `with torch.cuda.stream(ctx.stream)`)
     def _enter(self):
-        self.stream.wait_stream(torch.cuda.current_stream(self.device))
+        current = torch.cuda.current_stream(self.device)
+        if current.cuda_stream != self.stream.cuda_stream:
+            self.stream.wait_stream(current)
 
     def _exit(self):
-        torch.cuda.current_stream(self.device).wait_stream(self.stream)
+        current = torch.cuda.current_stream(self.device)
+        if current.cuda_stream != self.stream.cuda_stream:
+            current.wait_stream(self.stream)
 
     def sync(self):
         check(lib().flux2mi_ctx_sync(self.handle))
@@ -497,6 +513,161 @@ class Context:
         check(lib().flux2mi_op_attention_prescaled_range(self.handle, _ptr(qkv), _ptr(out), s, heads, float(score_bound_log2), q0, nq, nk))
         self._exit()
         return out
+
+    # ---- microscaled 4-bit floating point and the residual norm: row strides are taken as they are, the last dimension must be dense
+    def _matrix(self, t: torch.Tensor, dtypes, name: str, written: bool = False) -> Tuple[torch.Tensor, int]:
+        """A 2-D tensor on this context's GPU and its row stride in elements; a layout without dense rows is copied (refused if `written`)."""
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must be a tensor on {self.device}")
+        if t.dtype not in dtypes:
+            raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+        if t.dim() != 2:
+            raise Flux2Error(L.ERR_SHAPE, f"{name} must have two dimensions, got {tuple(t.shape)}")
+        rows, cols = t.shape
+        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+            if written:
+                raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must have dense rows, got strides {t.stride()}")
+            t = t.contiguous()
+        return t, t.stride(0) if rows > 1 else max(cols, 1)
+
+    def _vector(self, t: Optional[torch.Tensor], dtype, n: int, name: str) -> Optional[torch.Tensor]:
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != dtype:
+            raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must be a {dtype} tensor on {self.device}")
+        if t.dim() != 1 or t.shape[0] != n:
+            raise Flux2Error(L.ERR_SHAPE, f"{name} must have shape ({n},), got {tuple(t.shape)}")
+        return t.contiguous()
+
+    def _mxfp4(self, m: MXFP4, name: str) -> MXFP4:
+        codes, scales, cols = m
+        pad = -(-int(cols) // 128) * 128
+        for t, what, width in ((codes, "codes", pad // 2), (scales, "scales", pad // 32)):
+            if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.uint8:
+                raise Flux2Error(L.ERR_INVALID_ARG, f"{name}.{what} must be a torch.uint8 tensor on {self.device}")
+            if cols < 1 or t.dim() != 2 or t.shape != (codes.shape[0], width):
+                raise Flux2Error(L.ERR_SHAPE, f"{name}.{what} must have shape ({codes.shape[0]}, {width}) for {cols} columns, got {tuple(t.shape)}")
+        return MXFP4(codes.contiguous(), scales.contiguous(), int(cols))
+
+    def op_quantize_mxfp4(self, x: torch.Tensor) -> MXFP4:
+        """x f32 / bf16 / f16 [rows, cols] -> MXFP4 (one power of two per 32 values of a row, e2m1 codes, nearest-even)."""
+        x, ldx = self._matrix(x, tuple(_DT), "x")
+        rows, cols = x.shape
+        if cols < 1:
+            raise Flux2Error(L.ERR_SHAPE, "x has no columns")
+        pad = -(-cols // 128) * 128
+        codes = torch.empty((rows, pad // 2), dtype=torch.uint8, device=self.device)
+        scales = torch.empty((rows, pad // 32), dtype=torch.uint8, device=self.device)
+        self._enter()
+        check(lib().flux2mi_op_quantize_mxfp4(self.handle, _ptr(x), _DT[x.dtype], ldx, rows, cols, _ptr(codes), _ptr(scales)))
+        self._exit()
+        return MXFP4(codes, scales, cols)
+
+    def op_dequantize_mxfp4(self, m: MXFP4, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values of `m` (exact in float32 and bfloat16)."""
+        m = self._mxfp4(m, "m")
+        if dtype not in _DT:
+            raise Flux2Error(L.ERR_INVALID_ARG, f"dtype {dtype}")
+        out, ldo = self._out(out, m.rows, m.cols, dtype)
+        self._enter()
+        check(lib().flux2mi_op_dequantize_mxfp4(self.handle, _ptr(m.codes), _ptr(m.scales), m.rows, m.cols, _ptr(out), _DT[dtype], ldo))
+        self._exit()
+        return out
+
+    def _out(self, out: Optional[torch.Tensor], rows: int, cols: int, dtype) -> Tuple[torch.Tensor, int]:
+        if out is None:
+            return torch.empty((rows, cols), dtype=dtype, device=self.device), cols
+        out, ldo = self._matrix(out, (dtype,), "out", written=True)
+        if tuple(out.shape) != (rows, cols):
+            raise Flux2Error(L.ERR_SHAPE, f"out must have shape ({rows}, {cols}), got {tuple(out.shape)}")
+        return out, ldo
+
+    def _gemm_mxfp4(self, call, m: int, k: int, w: MXFP4, bias, gate, resid, dtype, out) -> torch.Tensor:
+        w = self._mxfp4(w, "w")
+        if w.cols != k:
+            raise Flux2Error(L.ERR_SHAPE, f"w has {w.cols} columns, a has {k}")
+        n = w.rows
+        bias, gate = self._vector(bias, torch.float32, n, "bias"), self._vector(gate, torch.float32, n, "gate")
+        ldr = n
+        if resid is not None:
+            if dtype not in (None, torch.float32):
+                raise Flux2Error(L.ERR_INVALID_ARG, "a residual needs a float32 output")
+            dtype = torch.float32
+            given = resid
+            resid, ldr = self._matrix(resid, (torch.float32,), "resid")
+            if tuple(resid.shape) != (m, n):
+                raise Flux2Error(L.ERR_SHAPE, f"resid must have shape ({m}, {n}), got {tuple(resid.shape)}")
+            if out is given:
+                resid = out
+        dtype = torch.bfloat16 if dtype is None else dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise Flux2Error(L.ERR_INVALID_ARG, f"dtype {dtype} (float32 or bfloat16)")
+        out, ldo = self._out(out, m, n, dtype)
+        self._enter()
+        check(call(_ptr(w.codes), _ptr(w.scales), _ptr(bias), _ptr(gate), _ptr(resid), ldr, _ptr(out), _DT[dtype], ldo, m, n, k))
+        self._exit()
+        return out
+
+    def op_gemm_mxfp4(self, a: MXFP4, w: MXFP4, bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                      resid: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """resid + gate * (a @ w.T + bias), both operands in MXFP4; bias, gate float32 [N], resid float32 [M, N] (each optional).
+        dtype: bfloat16 (default) or float32; float32 with resid.  out may be resid: x += gate * y in place."""
+        a = self._mxfp4(a, "a")
+        return self._gemm_mxfp4(lambda *r: lib().flux2mi_op_gemm_mxfp4(self.handle, _ptr(a.codes), _ptr(a.scales), *r),
+                                a.rows, a.cols, w, bias, gate, resid, dtype, out)
+
+    def op_gemm_bf16_mxfp4(self, a: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                           resid: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The same with a in bfloat16 [M, K]: only the weights are in 4 bits."""
+        a, lda = self._matrix(a, (torch.bfloat16,), "a")
+        return self._gemm_mxfp4(lambda *r: lib().flux2mi_op_gemm_bf16_mxfp4(self.handle, _ptr(a), lda, *r),
+                                a.shape[0], a.shape[1], w, bias, gate, resid, dtype, out)
+
+    _NORMS = {"none": L.NORM_NONE, "rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+
+    def op_residual_norm(self, x: torch.Tensor, y: Optional[torch.Tensor] = None, *, x_out: Optional[torch.Tensor] = None, split: int = 0,
+                         post_norm: str = "none", post_weight: Optional[torch.Tensor] = None, post_eps: float = 1e-6, gate=None,
+                         resid_scale: float = 1.0, norm: str = "rms", weight: Optional[torch.Tensor] = None, eps: float = 1e-6, shift=None,
+                         scale=None, dtype: torch.dtype = torch.bfloat16, want_out: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """x' = resid_scale * x + gate * (norm_post(y) * post_weight);  out = norm(x') * weight * (1 + scale) + shift.
+        x float32 [rows, dim], y bfloat16 / float32 or None; norms "none" | "rms" | "layer"; weights bfloat16 [dim]; gate, scale, shift
+        float32 [dim], or a pair of them: the first for rows < split.  x' goes to x_out, by default into x itself.
+        -> (x', out): out of `dtype` (bfloat16 / float32), None without want_out."""
+        x, ldx = self._matrix(x, (torch.float32,), "x", written=x_out is None)
+        rows, dim = x.shape
+        p = L.ResidualNorm(rows=rows, dim=dim, split=int(split), post_eps=post_eps, eps=eps, resid_scale=resid_scale, x=_ptr(x), ldx=ldx)
+        if post_norm not in self._NORMS or norm not in self._NORMS:
+            raise Flux2Error(L.ERR_INVALID_ARG, f"norms are {sorted(self._NORMS)}, got {post_norm!r}, {norm!r}")
+        p.post_norm, p.norm = self._NORMS[post_norm], self._NORMS[norm]
+        if y is not None:
+            y, p.ldy = self._matrix(y, (torch.float32, torch.bfloat16), "y")
+            if y.shape != x.shape:
+                raise Flux2Error(L.ERR_SHAPE, f"y must have shape {tuple(x.shape)}, got {tuple(y.shape)}")
+            p.y, p.y_dtype = _ptr(y), _DT[y.dtype]
+        if x_out is None:
+            x_out, p.ldx_out = x, ldx
+        else:
+            x_out, p.ldx_out = self._out(x_out, rows, dim, torch.float32)
+        p.x_out = _ptr(x_out)
+        keep = [self._vector(post_weight, torch.bfloat16, dim, "post_weight"), self._vector(weight, torch.bfloat16, dim, "weight")]
+        p.post_weight, p.weight = _ptr(keep[0]), _ptr(keep[1])
+        for name, v in (("gate", gate), ("scale", scale), ("shift", shift)):
+            pair = tuple(v) if isinstance(v, (tuple, list)) else (v, v)
+            if len(pair) != 2:
+                raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must be one vector or a pair")
+            pair = [self._vector(t, torch.float32, dim, name) for t in pair]
+            keep += pair
+            setattr(p, name, (C.c_void_p * 2)(*[_ptr(t) for t in pair]))
+        out = None
+        if want_out:
+            if dtype not in (torch.float32, torch.bfloat16):
+                raise Flux2Error(L.ERR_INVALID_ARG, f"dtype {dtype} (float32 or bfloat16)")
+            out = torch.empty((rows, dim), dtype=dtype, device=self.device)
+            p.out, p.out_dtype, p.ldo = _ptr(out), _DT[dtype], dim
+        self._enter()
+        check(lib().flux2mi_op_residual_norm(self.handle, C.byref(p)))
+        self._exit()
+        return x_out, out
 
 
 def _set_tensors(fn, handle, tensors: Dict[str, torch.Tensor]):

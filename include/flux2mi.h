@@ -579,6 +579,57 @@ int flux2mi_op_attention_qk8_blocks(flux2mi_ctx* ctx, const void* q8, const void
 int flux2mi_op_attention_prescaled_range(flux2mi_ctx* ctx, const void* qkv, void* out, int S, int heads, float score_bound_log2,
                                          int q0, int nq, int nk);
 
+/* ---- microscaled 4-bit floating point (MXFP4) ------------------------------------------------------------------------------
+ * The reference quantises weights to 4 or 8 bits with MLX's affine groups (Configuration/QuantizationConfig.swift:40-73,
+ * Flux2Pipeline.swift:573); these operators are this library's own 4-bit form, the one the matrix pipe multiplies natively (OCP
+ * Microscaling Formats, MXFP4).  A matrix [rows, cols] is cut into blocks of 32 consecutive values of a row.  A block keeps one
+ * byte, the scale 2^(byte - 127), and 32 codes of e2m1, values +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}:
+ *   byte = max(floor(log2 max|x|) - 2 + 127, 0), 0 for an all-zero block;  code = x / scale to the nearest value, ties to the even
+ *   code, beyond 6 to +-6.  A block that holds a NaN or an infinity: byte 255, codes 0 — it reads back as NaN, and products with it are NaN.
+ * Memory (device): codes u8 [rows][P / 2], two codes per byte, the even column in the low half; scales u8 [rows][P / 32]; P = cols
+ * rounded up to a multiple of 128.  The padding is written as zeros, and a matrix from elsewhere must hold zeros there.  codes must
+ * be 16-byte, scales 4-byte aligned.  Inputs and outputs of a call must not overlap unless said otherwise; rows, M or N of 0 do
+ * nothing.  All calls are async on the context's stream, allocate nothing and may be captured into a graph. */
+int64_t flux2mi_mxfp4_code_bytes(int64_t rows, int64_t cols);     /* rows * P / 2; 0 for invalid sizes */
+int64_t flux2mi_mxfp4_scale_bytes(int64_t rows, int64_t cols);    /* rows * P / 32 */
+/* x [rows, cols] of dtype f32 / bf16 / f16, row stride ldx elements -> codes, scales.  Exact: one rounding per value. */
+int flux2mi_op_quantize_mxfp4(flux2mi_ctx* ctx, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* codes,
+                              uint8_t* scales);
+/* the values the codes stand for: exact in f32 and bf16, rounded once to f16 */
+int flux2mi_op_dequantize_mxfp4(flux2mi_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y,
+                                int dtype, int64_t ldy);
+/* out [M, N] = resid + gate * (A W^T + bias): A [M, K] and W [N, K] in MXFP4, v_mfma_scale_f32_16x16x128_f8f6f4, f32 sums.
+ * bias, gate f32 [N], resid f32 [M, N] (row stride ld_resid): each may be NULL.  out f32 or bf16 (f32 with resid), row stride ld_out;
+ * out may be resid itself (x += gate * y, as flux2mi_op_gemm_gate_resid). */
+int flux2mi_op_gemm_mxfp4(flux2mi_ctx* ctx, const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
+                          const float* bias, const float* gate, const float* resid, int64_t ld_resid, void* out, int out_dtype,
+                          int64_t ld_out, int M, int N, int K);
+/* the same with A in bf16 [M, K], row stride lda: only the weights are in 4 bits (they become bf16 exactly, in registers) */
+int flux2mi_op_gemm_bf16_mxfp4(flux2mi_ctx* ctx, const void* a, int64_t lda, const uint8_t* w, const uint8_t* w_scales,
+                               const float* bias, const float* gate, const float* resid, int64_t ld_resid, void* out, int out_dtype,
+                               int64_t ld_out, int M, int N, int K);
+
+/* ---- the norms behind and in front of a block, fused with its gate and the residual's scale ----------------------------------
+ *   u  = norm_post(y) * post_weight          what the block returned, normalised
+ *   x' = resid_scale * x + gate * u          the residual stream (Flux2TransformerBlock.swift:117-166 applyGate + residual)
+ *   out = norm(x') * weight * (1 + scale) + shift      the operand of what comes next (:95-106, Flux2Modulation.swift:96-112)
+ * for blocks whose output is normalised before it joins the stream — that norm needs whole rows, so it cannot ride in the GEMM's
+ * gate + residual epilogue — and for the plain gate + residual + norm between two blocks.  One pass over x and y, f32 statistics. */
+enum { FLUX2MI_NORM_NONE = 0, FLUX2MI_NORM_RMS = 1, FLUX2MI_NORM_LAYER = 2 };
+typedef struct flux2mi_residual_norm {
+    int rows, dim;               /* rows < 2^24, dim <= 16384 */
+    int split;                   /* rows < split take gate[0], scale[0], shift[0]; the others [1] (text / image rows) */
+    int post_norm, norm;         /* FLUX2MI_NORM_* of y and of x' */
+    float post_eps, eps, resid_scale;
+    const float* x; int64_t ldx; /* f32 [rows, dim]; strides in elements */
+    const void* y; int y_dtype; int64_t ldy;         /* f32 / bf16 [rows, dim], or NULL: x' = resid_scale * x */
+    float* x_out; int64_t ldx_out;                   /* x', or NULL: not kept; may be x itself */
+    void* out; int out_dtype; int64_t ldo;           /* f32 / bf16, or NULL: only x' is wanted */
+    const void *post_weight, *weight;                /* bf16 [dim] or NULL (1) */
+    const float *gate[2], *scale[2], *shift[2];      /* f32 [dim] or NULL (gate 1, scale 0, shift 0) */
+} flux2mi_residual_norm;
+int flux2mi_op_residual_norm(flux2mi_ctx* ctx, const flux2mi_residual_norm* p);
+
 #ifdef __cplusplus
 }
 #endif
