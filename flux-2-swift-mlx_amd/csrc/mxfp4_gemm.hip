@@ -6,6 +6,8 @@
 // Operand layout (both forms): lane l of a wave holds row l % 16 of its 16-row block and the 32 values 32 (l / 16) ... of a 128-value step:
 // 16 bytes of codes = one MXFP4 block, so a lane needs one 16-byte load and one scale byte per step.  W is the MFMA's first operand: the
 // accumulator then holds 4 consecutive columns of one output row per lane (16-byte f32 / 8-byte bf16 stores).
+#include <utility>
+
 #include "dev.h"
 #include "mxfp4.h"
 
@@ -140,22 +142,49 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int t
 // step's into the other; the hand-over of a stage (its DMA has landed, everybody has left the previous stage) lies between two phases, so a
 // stage's DMA has two whole phases to arrive:
 //   P0: mfma F0 (step 0), read F1 <- buffer 0     | hand-over: buffer 1 landed, buffer 0 free
-//   P1: mfma F1 (step 1), read F0 <- buffer 1,  DMA of the next group's stage 0 -> buffer 0
+//   P1: mfma F1 (step 1), read F0 <- buffer 1,  DMA of the next group's stage 0 -> buffer 0 and of its scales
 //   P2: mfma F0 (step 2), read F1 <- buffer 1     | hand-over: buffer 0 landed, buffer 1 free
 //   P3: mfma F1 (step 3), read F0 <- buffer 0,  DMA of the next group's stage 1 -> buffer 1, scales of the next group
+// With one wave per SIMD every instruction takes an issue slot of ~5 cycles and an MFMA 16, so the side work goes between single MFMAs ("slots"),
+// at most two or three instructions at a time.
 // A lane's four scale bytes of a group (one per step) are gathered into one register, the byte is chosen by the MFMA's op_sel.
-// Steps behind K: addresses are clamped into the row and both scale bytes are 0, 2^-254 times finite codes, which is below f32: exactly 0.
+// Steps behind K: addresses stay inside the row and both scale bytes are 0, 2^-254 times finite codes, which is below f32: exactly 0.
 //
 // The MFMA is asm with the accumulator pinned to AGPRs: left to itself the register allocator of a one-wave-per-SIMD kernel moves accumulators
 // and fragments between the two files (492 copies per 256 MFMAs).  What the compiler then does not see are wait states: fragments come from LDS
 // (behind the compiler's own waits), scale registers pass through settle(), an accumulator is used again 16 or more MFMAs later and read behind drain().
+#define MFMA_FP4(SEL) "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4"
+#define SEL0 "op_sel_hi:[0,0,0]"
+#define SEL1 "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+#define SEL2 "op_sel_hi:[1,1,0]"
+#define SEL3 "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
 template <int OP>
 __device__ __forceinline__ void mfma_fp4_step(u32x4 w, u32x4 a, f32x4& c, uint32_t sw, uint32_t sa) {
-    if constexpr (OP == 0) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
-    if constexpr (OP == 1) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
-    if constexpr (OP == 2) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0] cbsz:4 blgp:4" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
-    if constexpr (OP == 3) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0] cbsz:4 blgp:4" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+    if constexpr (OP == 0) asm volatile(MFMA_FP4(SEL0) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+    if constexpr (OP == 1) asm volatile(MFMA_FP4(SEL1) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+    if constexpr (OP == 2) asm volatile(MFMA_FP4(SEL2) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+    if constexpr (OP == 3) asm volatile(MFMA_FP4(SEL3) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
 }
+// The same with a DMA piece around it: M0 is set in front of the MFMA (which is the wait state between the two), the request follows it.
+// 1 KB (256 B) per wave instruction: lane l's 16 (4) bytes at base + voff go to LDS at m0 + 16 (4) l.  As asm the DMA is not drained by the
+// compiler in front of every LDS read; it has no register result, and the hand-overs wait for it.
+template <int OP, bool CODES>
+__device__ __forceinline__ void mfma_fp4_dma(u32x4 w, u32x4 a, f32x4& c, uint32_t sw, uint32_t sa, uint32_t voff, const void* base, uint32_t lds) {
+#define WITH_DMA(SEL, LOAD) asm volatile("s_mov_b32 m0, %7\n\t" MFMA_FP4(SEL) "\n\t" LOAD " %5, %6" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "s"(lds) : "memory")
+    if constexpr (CODES) {
+        if constexpr (OP == 1) WITH_DMA(SEL1, "global_load_lds_dwordx4");
+        if constexpr (OP == 3) WITH_DMA(SEL3, "global_load_lds_dwordx4");
+    } else WITH_DMA(SEL1, "global_load_lds_dword");
+#undef WITH_DMA
+}
+__device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(uint32_t voff, const void* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+}
+// every piece requested so far has landed, and every wave's LDS reads have returned
+__device__ __forceinline__ void hand_over() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // wait states between the VALU instructions that made these registers and the asm MFMAs that read them
 template <int N>
 __device__ __forceinline__ void settle(uint32_t (&s)[N]) {
@@ -181,15 +210,10 @@ __device__ __forceinline__ void drain(f32x4 (&acc)[NT][MT]) {
         for (int i = 0; i < MT; ++i) asm volatile("" : "+a"(acc[j][i]));
 }
 
-// 1 KB per wave instruction: lane l's 16 (4) bytes at base + voff go to LDS at m0 + 16 (4) l.  Written as asm so that the compiler does not drain
-// the DMA in front of every LDS read; it has no register result, and the hand-overs below wait for it.
-__device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+template <class F, int... S>
+__device__ __forceinline__ void each_slot(F&& f, std::integer_sequence<int, S...>) {
+    (f(std::integral_constant<int, S>{}), ...);
 }
-__device__ __forceinline__ void dma4(uint32_t voff, const void* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
-}
-__device__ __forceinline__ void hand_over() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The tiles of one XCD (workgroups b, b + 8, ...) are neighbours: consecutive numbers within the XCD, walked in bands of `band` row tiles, so that
 // the A and W panels its workgroups share stay in its L2.
@@ -201,53 +225,90 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int ban
     tn = in / rows;
 }
 
-// A wave's 16 MT x 16 NT accumulators -> memory, 16 rows at a time through the wave's own LDS (the accumulator layout has one row per lane: stored
-// straight, every 8 or 16 bytes would be an access of their own; through LDS the lanes of an instruction cover whole row pieces).
-template <int MT, int NT, bool VEC>
+// A wave's 16 MT x 16 NT accumulators -> memory, 16 rows at a time through the wave's own LDS (two slots of 16 rows, so that a block is written
+// while the previous one is read): the accumulator layout has one row per lane, and stored straight, every 8 or 16 bytes would be an access of
+// their own; through LDS the lanes of an instruction cover whole row pieces.  A lane keeps its columns over all rows: bias and gate are read once.
+// The fields the loop uses are copied to opaque scalars: hipcc otherwise reads them from the kernel's arguments again at every use.
+template <int MT, int NT, bool BF16, bool VEC>
 __device__ __forceinline__ void store_tile(const Mxfp4Gemm& p, const f32x4 (&acc)[NT][MT], float* lds, int m0, int n0, int lane) {
-    constexpr int COLS = 16 * NT, PITCH = COLS + 4;
+    constexpr int COLS = 16 * NT, PITCH = COLS + 4, SLOT = 16 * PITCH;
     const int r = lane & 15, g = lane >> 4;
+    auto put = [&](int i) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+        for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(lds + (i & 1) * SLOT + r * PITCH + 16 * j + 4 * g) = acc[j][i];
+    };
+    auto ordered = [] {   // LDS executes a wave's accesses in order: only the compiler must keep them so
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+    };
+    put(0);
+    if constexpr (VEC) {
+        constexpr int CPL = BF16 ? 8 : 4, LPR = COLS / CPL, RPI = 64 / LPR, Q = 16 / RPI;   // columns per lane, lanes per row, rows per instruction
+        constexpr int ESZ = BF16 ? 2 : 4;
+        const int c = (lane % LPR) * CPL, n = n0 + c, row = lane / LPR;
+        const bool col_in = n < p.N;   // N % CPL == 0
+        int rows_left = p.M - m0 - row;
+        f32x4 bias[CPL / 4], gate[CPL / 4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(lds + r * PITCH + 16 * j + 4 * g) = acc[j][i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if constexpr (VEC) {
-            constexpr int LPR = COLS / 8, ROWS = 64 / LPR;   // lanes per row, 8 columns each; rows per instruction
-            const int c = (lane % LPR) * 8, n = n0 + c;
+        for (int h = 0; h < CPL / 4; ++h) {
+            bias[h] = p.bias && col_in ? *reinterpret_cast<const f32x4*>(p.bias + n + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
+            gate[h] = p.gate && col_in ? *reinterpret_cast<const f32x4*>(p.gate + n + 4 * h) : f32x4{1.f, 1.f, 1.f, 1.f};
+        }
+        if (!col_in) rows_left = 0;
+        uint64_t ld = (uint64_t)p.ld_out * ESZ, ldr = (uint64_t)p.ld_resid * 4;
+        const uint8_t* resid = reinterpret_cast<const uint8_t*>(p.resid);
+        uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
+        asm volatile("" : "+s"(ld), "+s"(ldr), "+s"(resid), "+s"(out));
+        uint8_t* o = out + (uint64_t)(m0 + row) * ld + (uint64_t)n * ESZ;
+        const uint8_t* x = resid + (uint64_t)(m0 + row) * ldr + (uint64_t)n * 4;
 #pragma unroll
-            for (int q = 0; q < 16 / ROWS; ++q) {
-                const int row = q * ROWS + lane / LPR, m = m0 + 16 * i + row;
-                const f32x4 lo = *reinterpret_cast<const f32x4*>(lds + row * PITCH + c), hi = *reinterpret_cast<const f32x4*>(lds + row * PITCH + c + 4);
-                if (p.out_bf16 && n + 8 <= p.N && !p.resid && p.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0) {
-                    if (m < p.M) {
-                        f32x4 a = lo, b = hi;
-                        if (p.bias) { a += *reinterpret_cast<const f32x4*>(p.bias + n); b += *reinterpret_cast<const f32x4*>(p.bias + n + 4); }
-                        if (p.gate) { a *= *reinterpret_cast<const f32x4*>(p.gate + n); b *= *reinterpret_cast<const f32x4*>(p.gate + n + 4); }
-                        const u32x4 u = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
-                        *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p.out) + m * p.ld_out + n) = u;
-                    }
-                } else {
-                    store4<true>(p, m, n, lo);
-                    store4<true>(p, m, n + 4, hi);
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) put(i + 1);
+            ordered();
+            f32x4 v[Q][CPL / 4];
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int h = 0; h < CPL / 4; ++h) v[q][h] = *reinterpret_cast<const f32x4*>(lds + (i & 1) * SLOT + (q * RPI + row) * PITCH + c + 4 * h);
+            f32x4 res[Q];
+            if (!BF16 && resid) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (16 * i + q * RPI < rows_left) res[q] = *reinterpret_cast<const f32x4*>(x + (uint64_t)(16 * i + q * RPI) * ldr);
+            }
+            ordered();
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+#pragma unroll
+                for (int h = 0; h < CPL / 4; ++h) v[q][h] = (v[q][h] + bias[h]) * gate[h];
+                if (16 * i + q * RPI < rows_left) {
+                    uint8_t* at = o + (uint64_t)(16 * i + q * RPI) * ld;
+                    if constexpr (BF16)
+                        *reinterpret_cast<u32x4*>(at) = u32x4{pack_bf16x2(v[q][0][0], v[q][0][1]), pack_bf16x2(v[q][0][2], v[q][0][3]),
+                                                              pack_bf16x2(v[q][CPL / 4 - 1][0], v[q][CPL / 4 - 1][1]), pack_bf16x2(v[q][CPL / 4 - 1][2], v[q][CPL / 4 - 1][3])};
+                    else *reinterpret_cast<f32x4*>(at) = resid ? v[q][0] + res[q] : v[q][0];
                 }
             }
-        } else {
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) put(i + 1);
+            ordered();
 #pragma unroll 4
             for (int q = 0; q < 16 * COLS / 64; ++q) {
                 const int at = q * 64 + lane, row = at / COLS, c = at % COLS;
-                store1(p, m0 + 16 * i + row, n0 + c, lds[row * PITCH + c]);
+                store1(p, m0 + 16 * i + row, n0 + c, lds[(i & 1) * SLOT + row * PITCH + c]);
             }
+            ordered();
         }
     }
 }
 
-template <int BM, int BN, bool VEC, int PER_CU>
+// TAIL: steps % 4 != 0, the last group is cut; otherwise DMA addresses need no per-lane arithmetic in the loop
+template <int BM, int BN, bool BF16, bool VEC, bool TAIL, int PER_CU>
 __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm p, int tiles_m, int tiles_n, int band) {
-    constexpr int MT = BM / 32, NT = BN / 32;              // 16-row blocks per wave
+    constexpr int MT = BM / 32, NT = BN / 32, SLOTS = MT * NT;   // 16-row blocks per wave; MFMAs per phase
     constexpr int ROWS = BM + BN;                          // LDS rows of a stage: W's, then A's
     constexpr int STAGE = ROWS * 128, SCALES = ROWS * 16;
     constexpr int PW = BN / 32, PA = BM / 32;              // code pieces per wave and stage
@@ -263,36 +324,28 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     const uint8_t* abase = reinterpret_cast<const uint8_t*>(p.a) + (int64_t)m0 * row_bytes;
     const uint8_t* wsbase = p.w_scales + (int64_t)n0 * row_scales;
     const uint8_t* asbase = p.a_scales + (int64_t)m0 * row_scales;
-    const int last_w = p.N - 1 - n0, last_a = p.M - 1 - m0;
+    const int last_w = p.N - 1 - n0, last_a = p.M - 1 - m0;   // rows behind the last one: its copy, never stored
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const int steps = p.steps, groups = (steps + 3) >> 2, last_stage = (steps - 1) >> 1;
 
-    // DMA sources: lane l fetches chunk (l % 8) ^ (row % 8) of row l / 8 of its piece
+    // DMA sources relative to the stage's (group's) column: lane l fetches chunk (l % 8) ^ (row % 8) of row l / 8 of its piece
     uint32_t vw[PW], va[PA], vsw[QW], vsa[QA];
     const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    const uint32_t quarter = TAIL ? 0u : (lane & 3) * 4u;
 #pragma unroll
-    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes; }
+    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes + chunk; }
 #pragma unroll
-    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes; }
+    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes + chunk; }
 #pragma unroll
-    for (int k = 0; k < QW; ++k) { const int row = (wave * QW + k) * 16 + (lane >> 2); vsw[k] = (uint32_t)(row < last_w ? row : last_w) * row_scales; }
+    for (int k = 0; k < QW; ++k) { const int row = (wave * QW + k) * 16 + (lane >> 2); vsw[k] = (uint32_t)(row < last_w ? row : last_w) * row_scales + quarter; }
 #pragma unroll
-    for (int k = 0; k < QA; ++k) { const int row = (wave * QA + k) * 16 + (lane >> 2); vsa[k] = (uint32_t)(row < last_a ? row : last_a) * row_scales; }
+    for (int k = 0; k < QA; ++k) { const int row = (wave * QA + k) * 16 + (lane >> 2); vsa[k] = (uint32_t)(row < last_a ? row : last_a) * row_scales + quarter; }
+    // the second step of the last stage may lie behind the row: its chunks are then fetched from the first step (their scales are 0)
+    auto back_of = [&](int stage) { return TAIL && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
+    auto step_of = [&](int group) { const int s = group * 4 + (lane & 3); return TAIL ? (uint32_t)(s < steps ? s : steps - 1) * 4u : 0u; };
+    auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + k) * 1024 : BN * 128 + (wave * PA + k - PW) * 1024); };
+    auto scale_lds = [&](int k, int group) { return lds0 + 2 * STAGE + (group & 1) * SCALES + (k < QW ? (wave * QW + k) * 256 : BN * 16 + (wave * QA + k - QW) * 256); };
 
-    const int groups = (p.steps + 3) >> 2;
-    // piece k of a stage (W's first); `cap`: the chunk's offset inside the row, clamped to its last one
-    auto dma_code = [&](int k, int stage, int buf, uint32_t live) {
-        uint32_t off = (uint32_t)stage * 128 + chunk;
-        off = off < row_bytes ? off : row_bytes - 16;
-        if (k < PW) dma16((vw[k] + off) & live, wbase, lds0 + buf * STAGE + (wave * PW + k) * 1024);
-        else dma16((va[k - PW] + off) & live, abase, lds0 + buf * STAGE + BN * 128 + (wave * PA + k - PW) * 1024);
-    };
-    auto dma_scale = [&](int k, int group, uint32_t live) {
-        int step = group * 4 + (lane & 3);
-        step = step < p.steps ? step : p.steps - 1;
-        const uint32_t at = lds0 + 2 * STAGE + (group & 1) * SCALES;
-        if (k < QW) dma4((vsw[k] + step * 4) & live, wsbase, at + (wave * QW + k) * 256);
-        else dma4((vsa[k - QW] + step * 4) & live, asbase, at + BN * 16 + (wave * QA + k - QW) * 256);
-    };
     // fragment reads
     const uint8_t* wrow = smem + (wn * NT * 16 + r) * 128;
     const uint8_t* arow = smem + (BN + wm * MT * 16 + r) * 128;
@@ -300,12 +353,14 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     auto frag_w = [&](int j, int buf, int ks) { return *reinterpret_cast<const u32x4*>(wrow + buf * STAGE + j * 2048 + (ks ? c1 : c0)); };
     auto frag_a = [&](int i, int buf, int ks) { return *reinterpret_cast<const u32x4*>(arow + buf * STAGE + i * 2048 + (ks ? c1 : c0)); };
     const uint32_t pick = (uint32_t)g | (uint32_t)(4 + g) << 8;
-    auto gather = [&](int row, int group) {   // byte s = scale of step s, block g; zero behind the last step
-        const u32x4 d = *reinterpret_cast<const u32x4*>(smem + 2 * STAGE + (group & 1) * SCALES + row * 16);
-        const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], pick), hi = __builtin_amdgcn_perm(d[3], d[2], pick);
-        const int left = p.steps - group * 4;
-        return __builtin_amdgcn_perm(hi, lo, 0x05040100u) & (left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1 : 0u);
+    auto scale_row = [&](int t, int group) {   // row block t of this wave, W's first: 16 bytes = 4 steps x 4 blocks
+        const int row = t < NT ? wn * NT * 16 + 16 * t + r : BN + wm * MT * 16 + 16 * (t - NT) + r;
+        return *reinterpret_cast<const u32x4*>(smem + 2 * STAGE + (group & 1) * SCALES + row * 16);
     };
+    auto gather = [&](u32x4 d, uint32_t live) {   // byte s = scale of step s, block g
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d[3], d[2], pick), __builtin_amdgcn_perm(d[1], d[0], pick), 0x05040100u) & live;
+    };
+    auto live_of = [&](int group) { const int left = steps - group * 4; return !TAIL || left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1 : 0u; };
 
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -316,58 +371,106 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     uint32_t sw[NT], sa[MT];
 
 #pragma unroll
-    for (int k = 0; k < QW + QA; ++k) dma_scale(k, 0, ~0u);
+    for (int k = 0; k < QW + QA; ++k) dma4((k < QW ? vsw[k] : vsa[k - QW]) + step_of(0), k < QW ? wsbase : asbase, scale_lds(k, 0));
 #pragma unroll
-    for (int k = 0; k < PW + PA; ++k) dma_code(k, 0, 0, ~0u);
+    for (int b = 0; b < 2; ++b) {
+        const int stage = b < last_stage ? b : last_stage;
 #pragma unroll
-    for (int k = 0; k < PW + PA; ++k) dma_code(k, 1, 1, ~0u);
+        for (int k = 0; k < PW + PA; ++k) dma16((k < PW ? vw[k] : va[k - PW]) - back_of(stage), (k < PW ? wbase : abase) + stage * 128, code_lds(k, b));
+    }
     hand_over();
 #pragma unroll
-    for (int j = 0; j < NT; ++j) { sw[j] = gather(wn * NT * 16 + 16 * j + r, 0); fw[0][j] = frag_w(j, 0, 0); }
+    for (int j = 0; j < NT; ++j) { sw[j] = gather(scale_row(j, 0), live_of(0)); fw[0][j] = frag_w(j, 0, 0); }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) { sa[i] = gather(BN + wm * MT * 16 + 16 * i + r, 0); fa[0][i] = frag_a(i, 0, 0); }
+    for (int i = 0; i < MT; ++i) { sa[i] = gather(scale_row(NT + i, 0), live_of(0)); fa[0][i] = frag_a(i, 0, 0); }
     settle(sw);
     settle(sa);
     settle_acc<MT, NT>(acc);
 
-    // one phase: MT row groups of NT MFMAs; the reads of the next step in the first half of them, DMA pieces spread over all
-#define PHASE(OP, CUR, NBUF, NKS, DMA)                                                                                         \
-    _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                           \
-        if (i < MT / 2) {                                                                                                      \
-            _Pragma("unroll") for (int t = i * (MT + NT) / (MT / 2); t < (i + 1) * (MT + NT) / (MT / 2); ++t) {                \
-                if (t < NT) fw[1 - CUR][t] = frag_w(t, NBUF, NKS);                                                             \
-                else fa[1 - CUR][t - NT] = frag_a(t - NT, NBUF, NKS);                                                          \
-            }                                                                                                                  \
-        }                                                                                                                      \
-        DMA;                                                                                                                   \
-        _Pragma("unroll") for (int j = 0; j < NT; ++j) mfma_fp4_step<OP>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i]); \
-        __builtin_amdgcn_sched_barrier(0);                                                                                     \
-    }
-#define CODES(STAGE_, BUF) _Pragma("unroll") for (int k = i * (PW + PA) / MT; k < (i + 1) * (PW + PA) / MT; ++k) dma_code(k, STAGE_, BUF, live);
-#define SCALE _Pragma("unroll") for (int k = i * (QW + QA) / MT; k < (i + 1) * (QW + QA) / MT; ++k) dma_scale(k, q + 1, live);
-    for (int q = 0; q < groups; ++q) {   // one body without a branch: behind the last group the requests all go to the operands' first bytes
-        const uint32_t live = q + 1 < groups ? 0xffffffffu : 0u;
-        PHASE(0, 0, 0, 1, )
-        hand_over();
-        PHASE(1, 1, 1, 0, CODES(2 * q + 2, 0) SCALE)
-        PHASE(2, 0, 1, 1, )
-        hand_over();
-        PHASE(3, 1, 0, 0, CODES(2 * q + 3, 1))
+    // One loop body without a branch: behind the last group the requests repeat that group's.
+    for (int q = 0; q < groups; ++q) {
+        const int qn = q + 1 < groups ? q + 1 : q;
+        const int s0 = 2 * qn, s1 = 2 * qn + 1 < last_stage ? 2 * qn + 1 : last_stage;
+        const uint8_t *w0 = wbase + s0 * 128, *a0 = abase + s0 * 128, *w1 = wbase + s1 * 128, *a1 = abase + s1 * 128;
+        const uint8_t *wsn = wsbase + (TAIL ? 0 : qn * 16), *asn = asbase + (TAIL ? 0 : qn * 16);
+        const uint32_t back0 = back_of(s0), back1 = back_of(s1), stepn = step_of(qn), live = live_of(q + 1);
+        u32x4 raw[NT + MT];   // (a few live at a time)
+        uint32_t nw[NT], na[MT];
+        auto phase = [&](auto op) {
+            constexpr int OP = decltype(op)::value, CUR = OP & 1, NBUF = OP == 1 || OP == 2 ? 1 : 0, NKS = OP & 1 ? 0 : 1;
+            constexpr int READS = MT + NT, RSPAN = SLOTS / 2;                               // fragment reads: spread over the first half
+            constexpr int NC = OP & 1 ? PW + PA : 0, NS = OP == 1 ? QW + QA : 0, ND = NC + NS; // DMA pieces: spread over the whole phase
+            constexpr int GB = (MT + NT) / 4;                                               // scale rows of a quarter of P3
+            each_slot([&](auto slot) {
+                constexpr int S = decltype(slot)::value, i = S / NT, j = S % NT;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sw[j] = gather(wn * NT * 16 + 16 * j + r, q + 1);
+                for (int t = 0; t < READS; ++t)
+                    if (t * RSPAN / READS == S) {
+                        if (t < NT) fw[1 - CUR][t] = frag_w(t, NBUF, NKS);
+                        else fa[1 - CUR][t - NT] = frag_a(t - NT, NBUF, NKS);
+                    }
+                if constexpr (OP == 3) {   // scales of the next group: read in one quarter of the phase, gathered in the next
+                    constexpr int QUART = SLOTS / 4, qi = S / QUART, at = S % QUART;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = gather(BN + wm * MT * 16 + 16 * i + r, q + 1);
+                    for (int t = 0; t < GB; ++t)
+                        if (t * QUART / GB == at) {
+                            raw[qi * GB + t] = scale_row(qi * GB + t, q + 1);
+                            if (qi > 0) {
+                                constexpr int base = (qi > 0 ? qi - 1 : 0) * GB;
+                                const uint32_t v = gather(raw[base + t], live);
+                                if (base + t < NT) nw[base + t] = v;
+                                else na[base + t - NT] = v;
+                            }
+                        }
+                }
+                constexpr int d0 = S * ND / SLOTS, d1 = (S + 1) * ND / SLOTS;   // at most one piece per slot
+                static_assert(d1 - d0 <= 1, "more DMA pieces than slots");
+                if constexpr (d1 > d0) {
+                    // scale pieces go first: they are small and needed with the stage
+                    if constexpr (d0 < NS) {
+                        mfma_fp4_dma<OP, false>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i], (d0 < QW ? vsw[d0 < QW ? d0 : 0] : vsa[d0 < QW ? 0 : d0 - QW]) + stepn,
+                                                d0 < QW ? wsn : asn, scale_lds(d0, q + 1));
+                    } else {
+                        constexpr int k = d0 - NS;
+                        mfma_fp4_dma<OP, true>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i], (k < PW ? vw[k < PW ? k : 0] : va[k < PW ? 0 : k - PW]) - (OP == 1 ? back0 : back1),
+                                               OP == 1 ? (k < PW ? w0 : a0) : (k < PW ? w1 : a1), code_lds(k, OP == 1 ? 0 : 1));
+                    }
+                } else mfma_fp4_step<OP>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }, std::make_integer_sequence<int, SLOTS>{});
+            if constexpr (OP == 3) {
+#pragma unroll
+                for (int t = 3 * GB; t < 4 * GB; ++t) {
+                    const uint32_t v = gather(raw[t], live);
+                    if (t < NT) nw[t] = v;
+                    else na[t - NT] = v;
+                }
+            }
+        };
+        phase(std::integral_constant<int, 0>{});
+        hand_over();
+        phase(std::integral_constant<int, 1>{});
+        phase(std::integral_constant<int, 2>{});
+        hand_over();
+        phase(std::integral_constant<int, 3>{});
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sw[j] = nw[j];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] = na[i];
         settle(sw);
         settle(sa);
     }
-#undef PHASE
-#undef CODES
-#undef SCALE
     drain<MT, NT>(acc);
     hand_over();   // everybody has left the stages: their LDS becomes the epilogue's
-    store_tile<MT, NT, VEC>(p, acc, reinterpret_cast<float*>(smem) + wave * (16 * (NT * 16 + 4)), m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    store_tile<MT, NT, BF16, VEC>(p, acc, reinterpret_cast<float*>(smem) + wave * (2 * 16 * (NT * 16 + 4)), m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
 }
 
+// rows of out and resid take 16-byte accesses of the columns a lane of store_tile owns (8 of bf16, 4 of f32)
+bool wide_rows(const Mxfp4Gemm& p) {
+    auto ok = [](const void* q, int64_t ld, int cols) { return !q || (reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % cols == 0); };
+    const int cols = p.out_bf16 ? 8 : 4;
+    return p.N % cols == 0 && ok(p.out, p.ld_out, cols) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
+}
 bool four_columns(const Mxfp4Gemm& p) {
     auto ok = [](const void* q, int64_t ld, int esz) { return !q || (reinterpret_cast<uintptr_t>(q) % (4 * esz) == 0 && ld % 4 == 0); };
     return p.N % 4 == 0 && ok(p.out, p.ld_out, p.out_bf16 ? 2 : 4) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
@@ -383,18 +486,25 @@ int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-template <int BM, int BN, int PER_CU>
-int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
+template <int BM, int BN, int PER_CU, bool BF16, bool VEC, bool TAIL>
+int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
     if (tn * tm >= (1 << 24)) return 1;
     constexpr int LDS = 2 * (BM + BN) * (128 + 16);
-    const dim3 grid((unsigned)(tn * tm)), block(256);
-    const bool vec = four_columns(p);
-    const void* fn = vec ? (const void*)mxfp4_gemm_tile_kernel<BM, BN, true, PER_CU> : (const void*)mxfp4_gemm_tile_kernel<BM, BN, false, PER_CU>;
-    if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
-    if (vec) mxfp4_gemm_tile_kernel<BM, BN, true, PER_CU><<<grid, block, LDS, stream>>>(p, (int)tm, (int)tn, 6);
-    else mxfp4_gemm_tile_kernel<BM, BN, false, PER_CU><<<grid, block, LDS, stream>>>(p, (int)tm, (int)tn, 6);
+    const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, TAIL, PER_CU>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
+    fn<<<dim3((unsigned)(tn * tm)), dim3(256), LDS, stream>>>(p, (int)tm, (int)tn, 6);
     return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+template <int BM, int BN, int PER_CU>
+int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
+    const bool vec = wide_rows(p), tail = p.steps % 4 != 0;
+    if (p.out_bf16) {
+        if (vec) return tail ? launch_tile_form<BM, BN, PER_CU, true, true, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, true, true, false>(stream, p);
+        return tail ? launch_tile_form<BM, BN, PER_CU, true, false, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, true, false, false>(stream, p);
+    }
+    if (vec) return tail ? launch_tile_form<BM, BN, PER_CU, false, true, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, false, true, false>(stream, p);
+    return tail ? launch_tile_form<BM, BN, PER_CU, false, false, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, false, false, false>(stream, p);
 }
 
 }  // namespace
