@@ -135,8 +135,8 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int t
 
 // ---------------------------------------------------------------------------------------------- tiles staged through LDS (MXFP4 x MXFP4)
 // BM x BN outputs per workgroup of four waves (2 x 2), each BM/2 x BN/2.  A stage is 256 k = 128 bytes of every row; a group is two stages =
-// four 128-k steps = 16 scale bytes of every row.  Both come by LDS-DMA: code pieces of 8 rows x 128 bytes (the 16-byte chunk c of row r lies at
-// chunk c ^ (r & 7), so that the eight rows a fragment read touches at once sit in different banks), scale pieces of 16 rows x 16 bytes.
+// four 128-k steps = 16 scale bytes of every row.  The codes come by LDS-DMA: pieces of 8 rows x 128 bytes (the 16-byte chunk c of row r lies at
+// chunk c ^ (r & 7), so that the eight rows a fragment read touches at once sit in different banks).
 //
 // The loop body is one group in four phases, one MFMA step each.  While a phase multiplies the fragments of one register set it reads the next
 // step's into the other; the hand-over of a stage (its DMA has landed, everybody has left the previous stage) lies between two phases, so a
@@ -146,13 +146,13 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int t
 //   P2: mfma F0 (step 2), read F1 <- buffer 1     | hand-over: buffer 0 landed, buffer 1 free
 //   P3: mfma F1 (step 3), read F0 <- buffer 0,  DMA of the next group's stage 1 -> buffer 1, scales of the next group
 // With one wave per SIMD every instruction takes an issue slot of ~5 cycles and an MFMA 16, so the side work goes between single MFMAs ("slots"),
-// at most two or three instructions at a time.
-// A lane's four scale bytes of a group (one per step) are gathered into one register, the byte is chosen by the MFMA's op_sel.
+// about one instruction at a time (measured: what an instruction costs beyond that is 4 cycles each).
+// A lane's four scale bytes of a group (one per step) are one register, the byte is chosen by the MFMA's op_sel.
 // Steps behind K: addresses stay inside the row and both scale bytes are 0, 2^-254 times finite codes, which is below f32: exactly 0.
 //
 // The MFMA is asm with the accumulator pinned to AGPRs: left to itself the register allocator of a one-wave-per-SIMD kernel moves accumulators
 // and fragments between the two files (492 copies per 256 MFMAs).  What the compiler then does not see are wait states: fragments come from LDS
-// (behind the compiler's own waits), scale registers pass through settle(), an accumulator is used again 16 or more MFMAs later and read behind drain().
+// (behind waits that the compiler sees), so do the scale registers, an accumulator is used again 16 or more MFMAs later and read behind drain().
 #define MFMA_FP4(SEL) "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4"
 #define SEL0 "op_sel_hi:[0,0,0]"
 #define SEL1 "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
@@ -165,32 +165,28 @@ __device__ __forceinline__ void mfma_fp4_step(u32x4 w, u32x4 a, f32x4& c, uint32
     if constexpr (OP == 2) asm volatile(MFMA_FP4(SEL2) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
     if constexpr (OP == 3) asm volatile(MFMA_FP4(SEL3) : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
 }
-// The same with a DMA piece around it: M0 is set in front of the MFMA (which is the wait state between the two), the request follows it.
-// 1 KB (256 B) per wave instruction: lane l's 16 (4) bytes at base + voff go to LDS at m0 + 16 (4) l.  As asm the DMA is not drained by the
-// compiler in front of every LDS read; it has no register result, and the hand-overs wait for it.
-template <int OP, bool CODES>
+// The same with a DMA piece around it: 1 KB per wave instruction, lane l's 16 bytes at base + voff + 1024 PIECE go to LDS at m0 + 1024 PIECE + 16 l.
+// M0 is set with the first of four pieces, in front of the MFMA (which is the wait state between the two), and kept for the others: nothing else in
+// the loop touches it.  As asm the DMA is not drained by the compiler in front of every LDS read; it has no register result, and the hand-overs wait for it.
+template <int OP, int PIECE>
 __device__ __forceinline__ void mfma_fp4_dma(u32x4 w, u32x4 a, f32x4& c, uint32_t sw, uint32_t sa, uint32_t voff, const void* base, uint32_t lds) {
-#define WITH_DMA(SEL, LOAD) asm volatile("s_mov_b32 m0, %7\n\t" MFMA_FP4(SEL) "\n\t" LOAD " %5, %6" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "s"(lds) : "memory")
-    if constexpr (CODES) {
-        if constexpr (OP == 1) WITH_DMA(SEL1, "global_load_lds_dwordx4");
-        if constexpr (OP == 3) WITH_DMA(SEL3, "global_load_lds_dwordx4");
-    } else WITH_DMA(SEL1, "global_load_lds_dword");
+#define WITH_DMA(SEL)                                                                                                                       \
+    if constexpr (PIECE == 0) asm volatile("s_mov_b32 m0, %7\n\t" MFMA_FP4(SEL) "\n\tglobal_load_lds_dwordx4 %5, %6" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "s"(lds) : "memory"); \
+    else asm volatile(MFMA_FP4(SEL) "\n\tglobal_load_lds_dwordx4 %5, %6 offset:%7" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "i"(PIECE * 1024) : "memory")
+    if constexpr (OP == 1) { WITH_DMA(SEL1); }
+    if constexpr (OP == 3) { WITH_DMA(SEL3); }
 #undef WITH_DMA
 }
 __device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void dma4(uint32_t voff, const void* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
-}
-// every piece requested so far has landed, and every wave's LDS reads have returned
-__device__ __forceinline__ void hand_over() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// wait states between the VALU instructions that made these registers and the asm MFMAs that read them
-template <int N>
-__device__ __forceinline__ void settle(uint32_t (&s)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(s[i]));
-    asm volatile("s_nop 7" ::: "memory");
+// every LDS read has returned (a builtin: the compiler then adds no waits of its own in front of the uses)
+__device__ __forceinline__ void lds_returned() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+// every piece requested so far has landed, and every wave's LDS accesses are done
+__device__ __forceinline__ void hand_over() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt 0, lgkmcnt 0
+    asm volatile("s_barrier" ::: "memory");
 }
 template <int MT, int NT>
 __device__ __forceinline__ void settle_acc(f32x4 (&acc)[NT][MT]) {
@@ -227,49 +223,65 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int ban
 
 // A wave's 16 MT x 16 NT accumulators -> memory, 16 rows at a time through the wave's own LDS (two slots of 16 rows, so that a block is written
 // while the previous one is read): the accumulator layout has one row per lane, and stored straight, every 8 or 16 bytes would be an access of
-// their own; through LDS the lanes of an instruction cover whole row pieces.  A lane keeps its columns over all rows: bias and gate are read once.
+// their own; through LDS the lanes of an instruction cover whole row pieces.  bf16 is rounded in front of LDS (half the traffic).
 // The fields the loop uses are copied to opaque scalars: hipcc otherwise reads them from the kernel's arguments again at every use.
-template <int MT, int NT, bool BF16, bool VEC>
-__device__ __forceinline__ void store_tile(const Mxfp4Gemm& p, const f32x4 (&acc)[NT][MT], float* lds, int m0, int n0, int lane) {
-    constexpr int COLS = 16 * NT, PITCH = COLS + 4, SLOT = 16 * PITCH;
+template <int MT, int NT, bool BF16>
+constexpr int store_slot_bytes() { return 16 * (16 * NT * (BF16 ? 2 : 4) + (BF16 ? 32 : 16)); }   // row pitches that spread 16 rows over the banks
+
+template <int MT, int NT, bool BF16, bool VEC, bool AFFINE>
+__device__ __forceinline__ void store_tile(const Mxfp4Gemm& p, const f32x4 (&acc)[NT][MT], uint8_t* lds, int m0, int n0, int lane) {
+    constexpr int COLS = 16 * NT, SLOT = store_slot_bytes<MT, NT, BF16>(), PITCH = SLOT / 16, ESZ = BF16 ? 2 : 4;
     const int r = lane & 15, g = lane >> 4;
-    auto put = [&](int i) {
+    // bias and gate: bf16 takes them in front of its rounding, for the lane's accumulator columns; f32 behind LDS, where a lane keeps its columns
+    f32x4 bias[NT], gate[NT];
+    if constexpr (AFFINE && BF16) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(lds + (i & 1) * SLOT + r * PITCH + 16 * j + 4 * g) = acc[j][i];
+        for (int j = 0; j < NT; ++j) {
+            const int n = n0 + 16 * j + 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                bias[j][e] = p.bias && n + e < p.N ? p.bias[n + e] : 0.f;
+                gate[j][e] = p.gate && n + e < p.N ? p.gate[n + e] : 1.f;
+            }
+        }
+    }
+    auto put = [&](int i) {
+        uint8_t* at = lds + (i & 1) * SLOT + r * PITCH + 4 * g * ESZ;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            f32x4 v = acc[j][i];
+            if constexpr (AFFINE && BF16) v = (v + bias[j]) * gate[j];
+            if constexpr (BF16) *reinterpret_cast<uint2*>(at + 32 * j) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            else *reinterpret_cast<f32x4*>(at + 64 * j) = v;
+        }
     };
     auto ordered = [] {   // LDS executes a wave's accesses in order: only the compiler must keep them so
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
+    uint64_t ld = (uint64_t)p.ld_out * ESZ, ldr = (uint64_t)p.ld_resid * 4;
+    const uint8_t* resid = reinterpret_cast<const uint8_t*>(p.resid);
+    uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
+    asm volatile("" : "+s"(ld), "+s"(ldr), "+s"(resid), "+s"(out));
     put(0);
     if constexpr (VEC) {
-        constexpr int CPL = BF16 ? 8 : 4, LPR = COLS / CPL, RPI = 64 / LPR, Q = 16 / RPI;   // columns per lane, lanes per row, rows per instruction
-        constexpr int ESZ = BF16 ? 2 : 4;
+        constexpr int CPL = 16 / ESZ, LPR = COLS / CPL, RPI = 64 / LPR, Q = 16 / RPI;   // columns per lane, lanes per row, rows per instruction
         const int c = (lane % LPR) * CPL, n = n0 + c, row = lane / LPR;
-        const bool col_in = n < p.N;   // N % CPL == 0
-        int rows_left = p.M - m0 - row;
-        f32x4 bias[CPL / 4], gate[CPL / 4];
-#pragma unroll
-        for (int h = 0; h < CPL / 4; ++h) {
-            bias[h] = p.bias && col_in ? *reinterpret_cast<const f32x4*>(p.bias + n + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
-            gate[h] = p.gate && col_in ? *reinterpret_cast<const f32x4*>(p.gate + n + 4 * h) : f32x4{1.f, 1.f, 1.f, 1.f};
-        }
-        if (!col_in) rows_left = 0;
-        uint64_t ld = (uint64_t)p.ld_out * ESZ, ldr = (uint64_t)p.ld_resid * 4;
-        const uint8_t* resid = reinterpret_cast<const uint8_t*>(p.resid);
-        uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
-        asm volatile("" : "+s"(ld), "+s"(ldr), "+s"(resid), "+s"(out));
+        const int rows_left = n < p.N ? p.M - m0 - row : 0;   // N % CPL == 0
         uint8_t* o = out + (uint64_t)(m0 + row) * ld + (uint64_t)n * ESZ;
         const uint8_t* x = resid + (uint64_t)(m0 + row) * ldr + (uint64_t)n * 4;
+        f32x4 b4 = {0.f, 0.f, 0.f, 0.f}, g4 = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (AFFINE && !BF16) {
+            if (p.bias && n < p.N) b4 = *reinterpret_cast<const f32x4*>(p.bias + n);
+            if (p.gate && n < p.N) g4 = *reinterpret_cast<const f32x4*>(p.gate + n);
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if (i + 1 < MT) put(i + 1);
             ordered();
-            f32x4 v[Q][CPL / 4];
+            u32x4 v[Q];
 #pragma unroll
-            for (int q = 0; q < Q; ++q)
-#pragma unroll
-                for (int h = 0; h < CPL / 4; ++h) v[q][h] = *reinterpret_cast<const f32x4*>(lds + (i & 1) * SLOT + (q * RPI + row) * PITCH + c + 4 * h);
+            for (int q = 0; q < Q; ++q) v[q] = *reinterpret_cast<const u32x4*>(lds + (i & 1) * SLOT + (q * RPI + row) * PITCH + c * ESZ);
             f32x4 res[Q];
             if (!BF16 && resid) {
 #pragma unroll
@@ -279,26 +291,41 @@ __device__ __forceinline__ void store_tile(const Mxfp4Gemm& p, const f32x4 (&acc
             ordered();
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-#pragma unroll
-                for (int h = 0; h < CPL / 4; ++h) v[q][h] = (v[q][h] + bias[h]) * gate[h];
-                if (16 * i + q * RPI < rows_left) {
-                    uint8_t* at = o + (uint64_t)(16 * i + q * RPI) * ld;
-                    if constexpr (BF16)
-                        *reinterpret_cast<u32x4*>(at) = u32x4{pack_bf16x2(v[q][0][0], v[q][0][1]), pack_bf16x2(v[q][0][2], v[q][0][3]),
-                                                              pack_bf16x2(v[q][CPL / 4 - 1][0], v[q][CPL / 4 - 1][1]), pack_bf16x2(v[q][CPL / 4 - 1][2], v[q][CPL / 4 - 1][3])};
-                    else *reinterpret_cast<f32x4*>(at) = resid ? v[q][0] + res[q] : v[q][0];
-                }
+                if constexpr (AFFINE && !BF16) v[q] = __builtin_bit_cast(u32x4, (__builtin_bit_cast(f32x4, v[q]) + b4) * g4);
+                if (!BF16 && resid) v[q] = __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, v[q]) + res[q]);
+                if (16 * i + q * RPI < rows_left) *reinterpret_cast<u32x4*>(o + (uint64_t)(16 * i + q * RPI) * ld) = v[q];
             }
         }
-    } else {
+    } else {   // one column per lane
+        const int rows_left = p.M - m0;
+        float b1[COLS / 64], g1[COLS / 64];
+        if constexpr (AFFINE && !BF16) {
+#pragma unroll
+            for (int h = 0; h < COLS / 64; ++h) {
+                const int n = n0 + 64 * h + lane;
+                b1[h] = p.bias && n < p.N ? p.bias[n] : 0.f;
+                g1[h] = p.gate && n < p.N ? p.gate[n] : 1.f;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if (i + 1 < MT) put(i + 1);
             ordered();
 #pragma unroll 4
             for (int q = 0; q < 16 * COLS / 64; ++q) {
-                const int at = q * 64 + lane, row = at / COLS, c = at % COLS;
-                store1(p, m0 + 16 * i + row, n0 + c, lds[(i & 1) * SLOT + row * PITCH + c]);
+                const int row = q * 64 / COLS, c = q * 64 % COLS + lane, n = n0 + c;
+                static_assert(COLS % 64 == 0, "a row piece is whole lanes");
+                const uint8_t* at = lds + (i & 1) * SLOT + row * PITCH + c * ESZ;
+                if (16 * i + row < rows_left && n < p.N) {
+                    uint8_t* o = out + (uint64_t)(m0 + 16 * i + row) * ld + (uint64_t)n * ESZ;
+                    if constexpr (BF16) *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(at);
+                    else {
+                        float f = *reinterpret_cast<const float*>(at);
+                        if constexpr (AFFINE) f = (f + b1[q % (COLS / 64)]) * g1[q % (COLS / 64)];
+                        if (resid) f += *reinterpret_cast<const float*>(resid + (uint64_t)(m0 + 16 * i + row) * ldr + (uint64_t)n * 4);
+                        *reinterpret_cast<float*>(o) = f;
+                    }
+                }
             }
             ordered();
         }
@@ -311,8 +338,8 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     constexpr int MT = BM / 32, NT = BN / 32, SLOTS = MT * NT;   // 16-row blocks per wave; MFMAs per phase
     constexpr int ROWS = BM + BN;                          // LDS rows of a stage: W's, then A's
     constexpr int STAGE = ROWS * 128, SCALES = ROWS * 16;
-    constexpr int PW = BN / 32, PA = BM / 32;              // code pieces per wave and stage
-    constexpr int QW = BN / 64, QA = BM / 64;              // scale pieces per wave and group
+    constexpr int PW = BN / 32, PA = BM / 32, NP = PW + PA; // code pieces per wave and stage
+    constexpr int SR = ROWS / 256;                         // scale rows per thread
     extern __shared__ __align__(1024) uint8_t smem[];      // [2][STAGE] codes, [2][SCALES] scales
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
@@ -322,45 +349,79 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     const uint32_t row_bytes = (uint32_t)p.steps * 64, row_scales = (uint32_t)p.steps * 4;
     const uint8_t* wbase = p.w + (int64_t)n0 * row_bytes;
     const uint8_t* abase = reinterpret_cast<const uint8_t*>(p.a) + (int64_t)m0 * row_bytes;
-    const uint8_t* wsbase = p.w_scales + (int64_t)n0 * row_scales;
-    const uint8_t* asbase = p.a_scales + (int64_t)m0 * row_scales;
     const int last_w = p.N - 1 - n0, last_a = p.M - 1 - m0;   // rows behind the last one: its copy, never stored
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int steps = p.steps, groups = (steps + 3) >> 2, last_stage = (steps - 1) >> 1;
 
-    // DMA sources relative to the stage's (group's) column: lane l fetches chunk (l % 8) ^ (row % 8) of row l / 8 of its piece
-    uint32_t vw[PW], va[PA], vsw[QW], vsa[QA];
+    // DMA sources relative to the stage's column: lane l fetches chunk (l % 8) ^ (row % 8) of row l / 8 of its piece.  Four pieces share one M0: the
+    // instruction's offset goes to both addresses, so piece k of them starts 1024 k further in LDS and its source offset carries -1024 k (+ 3072 so
+    // that it stays unsigned; the scalar base is 3072 lower).
+    uint32_t vw[PW], va[PA];
     const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    const uint32_t quarter = TAIL ? 0u : (lane & 3) * 4u;
 #pragma unroll
-    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes + chunk; }
+    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes + chunk + 3072 - (k & 3) * 1024; }
 #pragma unroll
-    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes + chunk; }
-#pragma unroll
-    for (int k = 0; k < QW; ++k) { const int row = (wave * QW + k) * 16 + (lane >> 2); vsw[k] = (uint32_t)(row < last_w ? row : last_w) * row_scales + quarter; }
-#pragma unroll
-    for (int k = 0; k < QA; ++k) { const int row = (wave * QA + k) * 16 + (lane >> 2); vsa[k] = (uint32_t)(row < last_a ? row : last_a) * row_scales + quarter; }
+    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes + chunk + 3072 - (k & 3) * 1024; }
+    wbase -= 3072;
+    abase -= 3072;
     // the second step of the last stage may lie behind the row: its chunks are then fetched from the first step (their scales are 0)
     auto back_of = [&](int stage) { return TAIL && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
-    auto step_of = [&](int group) { const int s = group * 4 + (lane & 3); return TAIL ? (uint32_t)(s < steps ? s : steps - 1) * 4u : 0u; };
-    auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + k) * 1024 : BN * 128 + (wave * PA + k - PW) * 1024); };
-    auto scale_lds = [&](int k, int group) { return lds0 + 2 * STAGE + (group & 1) * SCALES + (k < QW ? (wave * QW + k) * 256 : BN * 16 + (wave * QA + k - QW) * 256); };
+    auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + (k & ~3)) * 1024 : BN * 128 + (wave * PA + ((k - PW) & ~3)) * 1024); };
 
-    // fragment reads
-    const uint8_t* wrow = smem + (wn * NT * 16 + r) * 128;
-    const uint8_t* arow = smem + (BN + wm * MT * 16 + r) * 128;
-    const int c0 = (g ^ (r & 7)) * 16, c1 = ((4 + g) ^ (r & 7)) * 16;
-    auto frag_w = [&](int j, int buf, int ks) { return *reinterpret_cast<const u32x4*>(wrow + buf * STAGE + j * 2048 + (ks ? c1 : c0)); };
-    auto frag_a = [&](int i, int buf, int ks) { return *reinterpret_cast<const u32x4*>(arow + buf * STAGE + i * 2048 + (ks ? c1 : c0)); };
-    const uint32_t pick = (uint32_t)g | (uint32_t)(4 + g) << 8;
-    auto scale_row = [&](int t, int group) {   // row block t of this wave, W's first: 16 bytes = 4 steps x 4 blocks
-        const int row = t < NT ? wn * NT * 16 + 16 * t + r : BN + wm * MT * 16 + 16 * (t - NT) + r;
-        return *reinterpret_cast<const u32x4*>(smem + 2 * STAGE + (group & 1) * SCALES + row * 16);
+    // Scales of a group: a thread loads the 16 bytes [step][block] of its rows, transposes them to one register per block with the steps as
+    // its bytes and writes [row / 64][block][row % 16][row / 16 % 4]: a fragment lane then reads the registers of four row blocks at once.
+    const uint8_t* srow[SR];
+#pragma unroll
+    for (int h = 0; h < SR; ++h) {
+        const int row = threadIdx.x + 256 * h, ra = row - BN;
+        srow[h] = row < BN ? p.w_scales + (int64_t)(n0 + (row < last_w ? row : last_w)) * row_scales
+                           : p.a_scales + (int64_t)(m0 + (ra < last_a ? ra : last_a)) * row_scales;
+    }
+    auto load_scales = [&](int h, int group) {
+        u32x4 d;
+        if constexpr (TAIL) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int step = group * 4 + s;
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(srow[h] + (step < steps ? step : steps - 1) * 4);
+                d[s] = step < steps ? v : 0u;
+            }
+        } else {
+            typedef u32x4 __attribute__((aligned(4))) u32x4_dword;
+            d = *reinterpret_cast<const u32x4_dword*>(srow[h] + group * 16);
+        }
+        return d;
     };
-    auto gather = [&](u32x4 d, uint32_t live) {   // byte s = scale of step s, block g
-        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d[3], d[2], pick), __builtin_amdgcn_perm(d[1], d[0], pick), 0x05040100u) & live;
+    auto write_scales = [&](int h, u32x4 d, int buf) {
+        const int row = threadIdx.x + 256 * h;
+        uint32_t* at = reinterpret_cast<uint32_t*>(smem + 2 * STAGE + buf * SCALES + (row >> 6) * 1024 + (row & 15) * 16 + (row >> 4 & 3) * 4);
+        const uint32_t t0 = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), t1 = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+        const uint32_t t2 = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), t3 = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+        at[0] = __builtin_amdgcn_perm(t2, t0, 0x05040100u);
+        at[64] = __builtin_amdgcn_perm(t2, t0, 0x07060302u);
+        at[128] = __builtin_amdgcn_perm(t3, t1, 0x05040100u);
+        at[192] = __builtin_amdgcn_perm(t3, t1, 0x07060302u);
     };
-    auto live_of = [&](int group) { const int left = steps - group * 4; return !TAIL || left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1 : 0u; };
+    // four row blocks of this wave, W's first
+    auto read_scales = [&](int t, int buf) {
+        const int quad = t < NT / 4 ? wn * (NT / 4) + t : BN / 64 + wm * (MT / 4) + t - NT / 4;
+        return *reinterpret_cast<const u32x4*>(smem + 2 * STAGE + buf * SCALES + quad * 1024 + g * 256 + r * 16);
+    };
+
+    // fragment reads: LDS bytes of this lane's chunk, per stage buffer and step (opaque, or hipcc recomputes them at every read)
+    typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+    uint32_t fbw[2][2], fba[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const uint32_t c = ((4 * ks + g) ^ (r & 7)) * 16;
+            fbw[b][ks] = lds0 + b * STAGE + (wn * NT * 16 + r) * 128 + c;
+            fba[b][ks] = lds0 + b * STAGE + (BN + wm * MT * 16 + r) * 128 + c;
+            asm volatile("" : "+v"(fbw[b][ks]), "+v"(fba[b][ks]));
+        }
+    auto frag_w = [&](int j, int buf, int ks) { return *reinterpret_cast<lds_u32x4*>((uintptr_t)(fbw[buf][ks] + j * 2048)); };
+    auto frag_a = [&](int i, int buf, int ks) { return *reinterpret_cast<lds_u32x4*>((uintptr_t)(fba[buf][ks] + i * 2048)); };
 
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -368,101 +429,91 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     u32x4 fw[2][NT], fa[2][MT];
-    uint32_t sw[NT], sa[MT];
+    u32x4 sc[(NT + MT) / 4];   // scale registers of the current group
+    auto sw = [&](int j) { return sc[j / 4][j % 4]; };
+    auto sa = [&](int i) { return sc[NT / 4 + i / 4][i % 4]; };
 
-#pragma unroll
-    for (int k = 0; k < QW + QA; ++k) dma4((k < QW ? vsw[k] : vsa[k - QW]) + step_of(0), k < QW ? wsbase : asbase, scale_lds(k, 0));
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         const int stage = b < last_stage ? b : last_stage;
 #pragma unroll
-        for (int k = 0; k < PW + PA; ++k) dma16((k < PW ? vw[k] : va[k - PW]) - back_of(stage), (k < PW ? wbase : abase) + stage * 128, code_lds(k, b));
+        for (int k = 0; k < NP; ++k)
+            dma16((k < PW ? vw[k] : va[k - PW]) - back_of(stage), (k < PW ? wbase : abase) + stage * 128 + (k & 3) * 1024, code_lds(k, b) + (k & 3) * 1024);
+    }
+#pragma unroll
+    for (int h = 0; h < SR; ++h) {
+        write_scales(h, load_scales(h, 0), 0);
+        write_scales(h, load_scales(h, groups > 1 ? 1 : 0), 1);
     }
     hand_over();
 #pragma unroll
-    for (int j = 0; j < NT; ++j) { sw[j] = gather(scale_row(j, 0), live_of(0)); fw[0][j] = frag_w(j, 0, 0); }
+    for (int t = 0; t < (NT + MT) / 4; ++t) sc[t] = read_scales(t, 0);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) { sa[i] = gather(scale_row(NT + i, 0), live_of(0)); fa[0][i] = frag_a(i, 0, 0); }
-    settle(sw);
-    settle(sa);
+    for (int j = 0; j < NT; ++j) fw[0][j] = frag_w(j, 0, 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) fa[0][i] = frag_a(i, 0, 0);
     settle_acc<MT, NT>(acc);
 
     // One loop body without a branch: behind the last group the requests repeat that group's.
     for (int q = 0; q < groups; ++q) {
-        const int qn = q + 1 < groups ? q + 1 : q;
+        const int qn = q + 1 < groups ? q + 1 : q, q2 = q + 2 < groups ? q + 2 : groups - 1;
         const int s0 = 2 * qn, s1 = 2 * qn + 1 < last_stage ? 2 * qn + 1 : last_stage;
         const uint8_t *w0 = wbase + s0 * 128, *a0 = abase + s0 * 128, *w1 = wbase + s1 * 128, *a1 = abase + s1 * 128;
-        const uint8_t *wsn = wsbase + (TAIL ? 0 : qn * 16), *asn = asbase + (TAIL ? 0 : qn * 16);
-        const uint32_t back0 = back_of(s0), back1 = back_of(s1), stepn = step_of(qn), live = live_of(q + 1);
-        u32x4 raw[NT + MT];   // (a few live at a time)
-        uint32_t nw[NT], na[MT];
+        const uint32_t back0 = back_of(s0), back1 = back_of(s1);
+        u32x4 raw[SR];                 // scale rows of group q + 2: requested in P1, there at the second hand-over, written in P3
+        u32x4 next[(NT + MT) / 4];     // scale registers of group q + 1
         auto phase = [&](auto op) {
             constexpr int OP = decltype(op)::value, CUR = OP & 1, NBUF = OP == 1 || OP == 2 ? 1 : 0, NKS = OP & 1 ? 0 : 1;
-            constexpr int READS = MT + NT, RSPAN = SLOTS / 2;                               // fragment reads: spread over the first half
-            constexpr int NC = OP & 1 ? PW + PA : 0, NS = OP == 1 ? QW + QA : 0, ND = NC + NS; // DMA pieces: spread over the whole phase
-            constexpr int GB = (MT + NT) / 4;                                               // scale rows of a quarter of P3
+            constexpr int READS = MT + NT, ND = OP & 1 ? NP : 0;
             each_slot([&](auto slot) {
                 constexpr int S = decltype(slot)::value, i = S / NT, j = S % NT;
+                // fragment reads in the first half, DMA pieces over the whole phase, from a third of a slot distance on
 #pragma unroll
                 for (int t = 0; t < READS; ++t)
-                    if (t * RSPAN / READS == S) {
+                    if (t * SLOTS / (2 * READS) == S) {
                         if (t < NT) fw[1 - CUR][t] = frag_w(t, NBUF, NKS);
                         else fa[1 - CUR][t - NT] = frag_a(t - NT, NBUF, NKS);
                     }
-                if constexpr (OP == 3) {   // scales of the next group: read in one quarter of the phase, gathered in the next
-                    constexpr int QUART = SLOTS / 4, qi = S / QUART, at = S % QUART;
+                if constexpr (OP == 1) {
 #pragma unroll
-                    for (int t = 0; t < GB; ++t)
-                        if (t * QUART / GB == at) {
-                            raw[qi * GB + t] = scale_row(qi * GB + t, q + 1);
-                            if (qi > 0) {
-                                constexpr int base = (qi > 0 ? qi - 1 : 0) * GB;
-                                const uint32_t v = gather(raw[base + t], live);
-                                if (base + t < NT) nw[base + t] = v;
-                                else na[base + t - NT] = v;
-                            }
-                        }
+                    for (int h = 0; h < SR; ++h)
+                        if (S == SLOTS / 2 + h) raw[h] = load_scales(h, q2);
                 }
-                constexpr int d0 = S * ND / SLOTS, d1 = (S + 1) * ND / SLOTS;   // at most one piece per slot
-                static_assert(d1 - d0 <= 1, "more DMA pieces than slots");
-                if constexpr (d1 > d0) {
-                    // scale pieces go first: they are small and needed with the stage
-                    if constexpr (d0 < NS) {
-                        mfma_fp4_dma<OP, false>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i], (d0 < QW ? vsw[d0 < QW ? d0 : 0] : vsa[d0 < QW ? 0 : d0 - QW]) + stepn,
-                                                d0 < QW ? wsn : asn, scale_lds(d0, q + 1));
-                    } else {
-                        constexpr int k = d0 - NS;
-                        mfma_fp4_dma<OP, true>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i], (k < PW ? vw[k < PW ? k : 0] : va[k < PW ? 0 : k - PW]) - (OP == 1 ? back0 : back1),
-                                               OP == 1 ? (k < PW ? w0 : a0) : (k < PW ? w1 : a1), code_lds(k, OP == 1 ? 0 : 1));
-                    }
-                } else mfma_fp4_step<OP>(fw[CUR][j], fa[CUR][i], acc[j][i], sw[j], sa[i]);
+                if constexpr (OP == 3) {
+#pragma unroll
+                    for (int h = 0; h < SR; ++h)
+                        if (S == SLOTS / 2 + 8 * h) write_scales(h, raw[h], q & 1);
+#pragma unroll
+                    for (int t = 0; t < (NT + MT) / 4; ++t)
+                        if (S == SLOTS / 2 + 1 + 2 * t) next[t] = read_scales(t, (q + 1) & 1);
+                }
+                constexpr int k = S * ND / SLOTS;
+                if constexpr (ND > 0 && (S + 1) * ND / SLOTS > k) {   // at most one piece per slot
+                    mfma_fp4_dma<OP, k & 3>(fw[CUR][j], fa[CUR][i], acc[j][i], sw(j), sa(i), (k < PW ? vw[k < PW ? k : 0] : va[k < PW ? 0 : k - PW]) - (OP == 1 ? back0 : back1),
+                                            OP == 1 ? (k < PW ? w0 : a0) : (k < PW ? w1 : a1), code_lds(k, OP == 1 ? 0 : 1));
+                } else mfma_fp4_step<OP>(fw[CUR][j], fa[CUR][i], acc[j][i], sw(j), sa(i));
                 __builtin_amdgcn_sched_barrier(0);
             }, std::make_integer_sequence<int, SLOTS>{});
-            if constexpr (OP == 3) {
-#pragma unroll
-                for (int t = 3 * GB; t < 4 * GB; ++t) {
-                    const uint32_t v = gather(raw[t], live);
-                    if (t < NT) nw[t] = v;
-                    else na[t - NT] = v;
-                }
-            }
         };
         phase(std::integral_constant<int, 0>{});
         hand_over();
         phase(std::integral_constant<int, 1>{});
+        lds_returned();
         phase(std::integral_constant<int, 2>{});
         hand_over();
+#pragma unroll
+        for (int h = 0; h < SR; ++h) asm volatile("" : "+v"(raw[h]));   // (they are there; a use further down would wait for younger DMA too)
         phase(std::integral_constant<int, 3>{});
+        lds_returned();
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sw[j] = nw[j];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = na[i];
-        settle(sw);
-        settle(sa);
+        for (int t = 0; t < (NT + MT) / 4; ++t) sc[t] = next[t];
+        asm volatile("s_nop 7" ::: "memory");   // (a copy of a scale register, if there is one, settles)
     }
     drain<MT, NT>(acc);
     hand_over();   // everybody has left the stages: their LDS becomes the epilogue's
-    store_tile<MT, NT, BF16, VEC>(p, acc, reinterpret_cast<float*>(smem) + wave * (2 * 16 * (NT * 16 + 4)), m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    uint8_t* mine = smem + wave * 2 * store_slot_bytes<MT, NT, BF16>();
+    if (p.bias || p.gate) store_tile<MT, NT, BF16, VEC, true>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    else store_tile<MT, NT, BF16, VEC, false>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
 }
 
 // rows of out and resid take 16-byte accesses of the columns a lane of store_tile owns (8 of bf16, 4 of f32)
