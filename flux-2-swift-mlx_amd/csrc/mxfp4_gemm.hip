@@ -139,12 +139,14 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int t
 // chunk c ^ (r & 7), so that the eight rows a fragment read touches at once sit in different banks).
 //
 // The loop body is one group in four phases, one MFMA step each.  While a phase multiplies the fragments of one register set it reads the next
-// step's into the other; the hand-over of a stage (its DMA has landed, everybody has left the previous stage) lies between two phases, so a
-// stage's DMA has two whole phases to arrive:
-//   P0: mfma F0 (step 0), read F1 <- buffer 0     | hand-over: buffer 1 landed, buffer 0 free
-//   P1: mfma F1 (step 1), read F0 <- buffer 1,  DMA of the next group's stage 0 -> buffer 0 and of its scales
-//   P2: mfma F0 (step 2), read F1 <- buffer 1     | hand-over: buffer 0 landed, buffer 1 free
-//   P3: mfma F1 (step 3), read F0 <- buffer 0,  DMA of the next group's stage 1 -> buffer 1, scales of the next group
+// step's into the other:
+//   P0: mfma F0 (step 0), read F1 <- buffer 0 in its first part, buffer 0 is free in its middle;  buffer 1 has landed at its end
+//   P1: mfma F1 (step 1), read F0 <- buffer 1
+//   P2: mfma F0 (step 2), read F1 <- buffer 1 in its first part, buffer 1 is free in its middle;  buffer 0 has landed at its end
+//   P3: mfma F1 (step 3), read F0 <- buffer 0
+// A buffer's next stage is requested from the moment it is free on, evenly, over one and a half phases; the other buffer's is then still in flight
+// and stays so over the hand-over.  (Requests in P1 and P3 alone, with nothing left in flight at a hand-over: 2 x 64 KB take 5100 cycles even
+// without an MFMA, against 2900 for a stream that is never drained and 4100 of the MFMAs.)
 // With one wave per SIMD every instruction takes an issue slot of ~5 cycles and an MFMA 16, so the side work goes between single MFMAs ("slots"),
 // about one instruction at a time (measured: what an instruction costs beyond that is 4 cycles each).
 // A lane's four scale bytes of a group (one per step) are one register, the byte is chosen by the MFMA's op_sel.
@@ -173,19 +175,26 @@ __device__ __forceinline__ void mfma_fp4_dma(u32x4 w, u32x4 a, f32x4& c, uint32_
 #define WITH_DMA(SEL)                                                                                                                       \
     if constexpr (PIECE == 0) asm volatile("s_mov_b32 m0, %7\n\t" MFMA_FP4(SEL) "\n\tglobal_load_lds_dwordx4 %5, %6" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "s"(lds) : "memory"); \
     else asm volatile(MFMA_FP4(SEL) "\n\tglobal_load_lds_dwordx4 %5, %6 offset:%7" : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa), "v"(voff), "s"(base), "i"(PIECE * 1024) : "memory")
+    if constexpr (OP == 0) { WITH_DMA(SEL0); }
     if constexpr (OP == 1) { WITH_DMA(SEL1); }
+    if constexpr (OP == 2) { WITH_DMA(SEL2); }
     if constexpr (OP == 3) { WITH_DMA(SEL3); }
 #undef WITH_DMA
 }
 __device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
 }
+__device__ __forceinline__ void dma4(uint32_t voff, const void* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+}
 // every LDS read has returned (a builtin: the compiler then adds no waits of its own in front of the uses)
 __device__ __forceinline__ void lds_returned() { __builtin_amdgcn_s_waitcnt(0xc07f); }
-// every piece requested so far has landed, and every wave's LDS accesses are done
+// every piece but the FLYING youngest has landed, and every wave's LDS accesses are done
+template <int FLYING>
 __device__ __forceinline__ void hand_over() {
+    static_assert(FLYING < 16, "the low four bits of vmcnt");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt 0, lgkmcnt 0
+    __builtin_amdgcn_s_waitcnt(0x0070 | FLYING);   // vmcnt FLYING, lgkmcnt 0
     asm volatile("s_barrier" ::: "memory");
 }
 template <int MT, int NT>
@@ -332,15 +341,19 @@ __device__ __forceinline__ void store_tile(const Mxfp4Gemm& p, const f32x4 (&acc
     }
 }
 
-// TAIL: steps % 4 != 0, the last group is cut; otherwise DMA addresses need no per-lane arithmetic in the loop
-template <int BM, int BN, bool BF16, bool VEC, bool TAIL, int PER_CU>
+// CUT: whether the last group is cut; if not, DMA addresses need no per-lane arithmetic in the loop
+enum { CUT_NONE = 0, CUT_TAIL = 1, CUT_SHORT = 2 };   // steps % 4 == 0, steps >= 4, steps < 4
+template <int BM, int BN, bool BF16, bool VEC, int CUT, int PER_CU>
 __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm p, int tiles_m, int tiles_n, int band) {
     constexpr int MT = BM / 32, NT = BN / 32, SLOTS = MT * NT;   // 16-row blocks per wave; MFMAs per phase
     constexpr int ROWS = BM + BN;                          // LDS rows of a stage: W's, then A's
     constexpr int STAGE = ROWS * 128, SCALES = ROWS * 16;
     constexpr int PW = BN / 32, PA = BM / 32, NP = PW + PA; // code pieces per wave and stage
+    // slot of P0 (P2) in which the buffer is free; piece k of its next stage goes with slot FREE + 1 + k EVERY, counted on into P1 (P3)
+    constexpr int FREE = SLOTS / 2, EVERY = SLOTS * 3 / 2 / NP, FIRST = (SLOTS - FREE - 2) / EVERY + 1;   // FIRST: pieces requested in P0 (P2)
+    static_assert(FREE + 1 + (NP - 1) * EVERY < 2 * SLOTS, "the last piece lies in the second phase");
     constexpr int SR = ROWS / 256;                         // scale rows per thread
-    extern __shared__ __align__(1024) uint8_t smem[];      // [2][STAGE] codes, [2][SCALES] scales
+    extern __shared__ __align__(1024) uint8_t smem[];      // [2][STAGE] codes, [2][SCALES] scales, [SCALES] scales as they came
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
     int tm, tn;
@@ -365,30 +378,45 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     wbase -= 3072;
     abase -= 3072;
     // the second step of the last stage may lie behind the row: its chunks are then fetched from the first step (their scales are 0)
-    auto back_of = [&](int stage) { return TAIL && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
+    auto back_of = [&](int stage) { return CUT != CUT_NONE && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
     auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + (k & ~3)) * 1024 : BN * 128 + (wave * PA + ((k - PW) & ~3)) * 1024); };
 
-    // Scales of a group: a thread loads the 16 bytes [step][block] of its rows, transposes them to one register per block with the steps as
-    // its bytes and writes [row / 64][block][row % 16][row / 16 % 4]: a fragment lane then reads the registers of four row blocks at once.
-    const uint8_t* srow[SR];
+    // Scales of a group: the 16 bytes [step][block] of row 64 wave + lane + 256 h come to LDS by DMA as they are; the same lane transposes them to
+    // one register per block with the steps as its bytes and writes [row / 64][block][row % 16][row / 16 % 4]: a fragment lane then reads the
+    // registers of four row blocks at once.  (Loaded into registers instead, their use makes the compiler wait for every younger DMA piece too:
+    // 4608 x 36864 x 4096 388 us, this way 360.)
+    uint32_t vs[SR];
+    const uint8_t* sbase[SR];
 #pragma unroll
     for (int h = 0; h < SR; ++h) {
-        const int row = threadIdx.x + 256 * h, ra = row - BN;
-        srow[h] = row < BN ? p.w_scales + (int64_t)(n0 + (row < last_w ? row : last_w)) * row_scales
-                           : p.a_scales + (int64_t)(m0 + (ra < last_a ? ra : last_a)) * row_scales;
+        const int first = wave * 64 + 256 * h, row = (first < BN ? first : first - BN) + lane;
+        vs[h] = (uint32_t)(first < BN ? (row < last_w ? row : last_w) : (row < last_a ? row : last_a)) * row_scales;
+        sbase[h] = first < BN ? p.w_scales + (int64_t)n0 * row_scales : p.a_scales + (int64_t)m0 * row_scales;
     }
-    auto load_scales = [&](int h, int group) {
+    constexpr int RAW = 2 * STAGE + 2 * SCALES;
+    // a cut group's 16 bytes are the row's last ones, `skip` steps in front of the group's own; rows of fewer than four steps come dword by dword
+    auto skip_of = [&](int group) { return CUT == CUT_TAIL && group * 4 + 4 > steps ? group * 4 + 4 - steps : 0; };
+    auto fetch_scales = [&](int h, int group) {
+        if constexpr (CUT == CUT_SHORT) {   // LDS: [step][row]
+#pragma unroll
+            for (int s = 0; s < 4; ++s) dma4(vs[h], sbase[h] + (s < steps ? s : steps - 1) * 4, lds0 + RAW + h * 4096 + s * 1024 + wave * 256);
+        } else dma16(vs[h], sbase[h] + (group * 4 - skip_of(group)) * 4, lds0 + RAW + (h * 256 + wave * 64) * 16);   // LDS: [row][step]
+    };
+    auto take_scales = [&](int h, int group) {   // steps behind K: 0
         u32x4 d;
-        if constexpr (TAIL) {
+        if constexpr (CUT == CUT_SHORT) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const int step = group * 4 + s;
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(srow[h] + (step < steps ? step : steps - 1) * 4);
-                d[s] = step < steps ? v : 0u;
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(smem + RAW + h * 4096 + s * 1024 + threadIdx.x * 4);
+                d[s] = s < steps ? v : 0u;
             }
         } else {
-            typedef u32x4 __attribute__((aligned(4))) u32x4_dword;
-            d = *reinterpret_cast<const u32x4_dword*>(srow[h] + group * 16);
+            d = *reinterpret_cast<const u32x4*>(smem + RAW + (h * 256 + threadIdx.x) * 16);
+            if constexpr (CUT == CUT_TAIL) {
+                const int skip = skip_of(group);
+                if (skip & 1) d = u32x4{d[1], d[2], d[3], 0u};
+                if (skip & 2) d = u32x4{d[2], d[3], 0u, 0u};
+            }
         }
         return d;
     };
@@ -441,11 +469,16 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
             dma16((k < PW ? vw[k] : va[k - PW]) - back_of(stage), (k < PW ? wbase : abase) + stage * 128 + (k & 3) * 1024, code_lds(k, b) + (k & 3) * 1024);
     }
 #pragma unroll
-    for (int h = 0; h < SR; ++h) {
-        write_scales(h, load_scales(h, 0), 0);
-        write_scales(h, load_scales(h, groups > 1 ? 1 : 0), 1);
-    }
-    hand_over();
+    for (int h = 0; h < SR; ++h) fetch_scales(h, 0);
+    hand_over<0>();
+#pragma unroll
+    for (int h = 0; h < SR; ++h) write_scales(h, take_scales(h, 0), 0);
+    lds_returned();
+#pragma unroll
+    for (int h = 0; h < SR; ++h) fetch_scales(h, groups > 1 ? 1 : 0);
+    hand_over<0>();
+#pragma unroll
+    for (int h = 0; h < SR; ++h) write_scales(h, take_scales(h, groups > 1 ? 1 : 0), 1);
 #pragma unroll
     for (int t = 0; t < (NT + MT) / 4; ++t) sc[t] = read_scales(t, 0);
 #pragma unroll
@@ -460,26 +493,28 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
         const int s0 = 2 * qn, s1 = 2 * qn + 1 < last_stage ? 2 * qn + 1 : last_stage;
         const uint8_t *w0 = wbase + s0 * 128, *a0 = abase + s0 * 128, *w1 = wbase + s1 * 128, *a1 = abase + s1 * 128;
         const uint32_t back0 = back_of(s0), back1 = back_of(s1);
-        u32x4 raw[SR];                 // scale rows of group q + 2: requested in P1, there at the second hand-over, written in P3
-        u32x4 next[(NT + MT) / 4];     // scale registers of group q + 1
+        // the scales of group q + 2 are requested in P1, have landed at the hand-over behind P2 and are transposed in P3, which reads those of group q + 1
+        u32x4 raw[SR], next[(NT + MT) / 4];
         auto phase = [&](auto op) {
             constexpr int OP = decltype(op)::value, CUR = OP & 1, NBUF = OP == 1 || OP == 2 ? 1 : 0, NKS = OP & 1 ? 0 : 1;
-            constexpr int READS = MT + NT, ND = OP & 1 ? NP : 0;
+            constexpr int READS = MT + NT, RSPAN = OP & 1 ? SLOTS / 2 : SLOTS * 3 / 8;
             each_slot([&](auto slot) {
                 constexpr int S = decltype(slot)::value, i = S / NT, j = S % NT;
-                // fragment reads in the first half, DMA pieces over the whole phase, from a third of a slot distance on
 #pragma unroll
                 for (int t = 0; t < READS; ++t)
-                    if (t * SLOTS / (2 * READS) == S) {
+                    if (t * RSPAN / READS == S) {
                         if (t < NT) fw[1 - CUR][t] = frag_w(t, NBUF, NKS);
                         else fa[1 - CUR][t - NT] = frag_a(t - NT, NBUF, NKS);
                     }
-                if constexpr (OP == 1) {
+                if constexpr (OP == 1) {   // in front of a piece that sets M0
 #pragma unroll
                     for (int h = 0; h < SR; ++h)
-                        if (S == SLOTS / 2 + h) raw[h] = load_scales(h, q2);
+                        if (S == FREE + 1 + NP / 2 * EVERY - SLOTS - 1 - h) fetch_scales(h, q2);
                 }
                 if constexpr (OP == 3) {
+#pragma unroll
+                    for (int h = 0; h < SR; ++h)
+                        if (S == SLOTS / 4 + h) raw[h] = take_scales(h, q2);
 #pragma unroll
                     for (int h = 0; h < SR; ++h)
                         if (S == SLOTS / 2 + 8 * h) write_scales(h, raw[h], q & 1);
@@ -487,22 +522,24 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
                     for (int t = 0; t < (NT + MT) / 4; ++t)
                         if (S == SLOTS / 2 + 1 + 2 * t) next[t] = read_scales(t, (q + 1) & 1);
                 }
-                constexpr int k = S * ND / SLOTS;
-                if constexpr (ND > 0 && (S + 1) * ND / SLOTS > k) {   // at most one piece per slot
-                    mfma_fp4_dma<OP, k & 3>(fw[CUR][j], fa[CUR][i], acc[j][i], sw(j), sa(i), (k < PW ? vw[k < PW ? k : 0] : va[k < PW ? 0 : k - PW]) - (OP == 1 ? back0 : back1),
-                                            OP == 1 ? (k < PW ? w0 : a0) : (k < PW ? w1 : a1), code_lds(k, OP == 1 ? 0 : 1));
+                if constexpr (!(OP & 1) && S == FREE) {   // everybody has read its last fragments of the buffer
+                    lds_returned();
+                    asm volatile("s_barrier" ::: "memory");
+                }
+                constexpr int since = (OP & 1 ? SLOTS : 0) + S - FREE - 1, k = since >= 0 && since % EVERY == 0 ? since / EVERY : NP;
+                if constexpr (k < NP) {
+                    mfma_fp4_dma<OP, k & 3>(fw[CUR][j], fa[CUR][i], acc[j][i], sw(j), sa(i), (k < PW ? vw[k < PW ? k : 0] : va[k < PW ? 0 : k - PW]) - (OP < 2 ? back0 : back1),
+                                            OP < 2 ? (k < PW ? w0 : a0) : (k < PW ? w1 : a1), code_lds(k, OP < 2 ? 0 : 1));
                 } else mfma_fp4_step<OP>(fw[CUR][j], fa[CUR][i], acc[j][i], sw(j), sa(i));
                 __builtin_amdgcn_sched_barrier(0);
             }, std::make_integer_sequence<int, SLOTS>{});
         };
         phase(std::integral_constant<int, 0>{});
-        hand_over();
+        hand_over<FIRST>();
         phase(std::integral_constant<int, 1>{});
         lds_returned();
         phase(std::integral_constant<int, 2>{});
-        hand_over();
-#pragma unroll
-        for (int h = 0; h < SR; ++h) asm volatile("" : "+v"(raw[h]));   // (they are there; a use further down would wait for younger DMA too)
+        hand_over<FIRST>();
         phase(std::integral_constant<int, 3>{});
         lds_returned();
 #pragma unroll
@@ -510,7 +547,7 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
         asm volatile("s_nop 7" ::: "memory");   // (a copy of a scale register, if there is one, settles)
     }
     drain<MT, NT>(acc);
-    hand_over();   // everybody has left the stages: their LDS becomes the epilogue's
+    hand_over<0>();   // everybody has left the stages: their LDS becomes the epilogue's
     uint8_t* mine = smem + wave * 2 * store_slot_bytes<MT, NT, BF16>();
     if (p.bias || p.gate) store_tile<MT, NT, BF16, VEC, true>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
     else store_tile<MT, NT, BF16, VEC, false>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
@@ -537,25 +574,27 @@ int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-template <int BM, int BN, int PER_CU, bool BF16, bool VEC, bool TAIL>
+template <int BM, int BN, int PER_CU, bool BF16, bool VEC, int CUT>
 int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
     if (tn * tm >= (1 << 24)) return 1;
-    constexpr int LDS = 2 * (BM + BN) * (128 + 16);
-    const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, TAIL, PER_CU>;
+    constexpr int LDS = (BM + BN) * (2 * 128 + 3 * 16);
+    const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, CUT, PER_CU>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
     fn<<<dim3((unsigned)(tn * tm)), dim3(256), LDS, stream>>>(p, (int)tm, (int)tn, 6);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
+template <int BM, int BN, int PER_CU, bool BF16, bool VEC>
+int launch_tile_cut(hipStream_t stream, const Mxfp4Gemm& p) {
+    if (p.steps < 4) return launch_tile_form<BM, BN, PER_CU, BF16, VEC, CUT_SHORT>(stream, p);
+    if (p.steps % 4) return launch_tile_form<BM, BN, PER_CU, BF16, VEC, CUT_TAIL>(stream, p);
+    return launch_tile_form<BM, BN, PER_CU, BF16, VEC, CUT_NONE>(stream, p);
+}
 template <int BM, int BN, int PER_CU>
 int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
-    const bool vec = wide_rows(p), tail = p.steps % 4 != 0;
-    if (p.out_bf16) {
-        if (vec) return tail ? launch_tile_form<BM, BN, PER_CU, true, true, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, true, true, false>(stream, p);
-        return tail ? launch_tile_form<BM, BN, PER_CU, true, false, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, true, false, false>(stream, p);
-    }
-    if (vec) return tail ? launch_tile_form<BM, BN, PER_CU, false, true, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, false, true, false>(stream, p);
-    return tail ? launch_tile_form<BM, BN, PER_CU, false, false, true>(stream, p) : launch_tile_form<BM, BN, PER_CU, false, false, false>(stream, p);
+    const bool vec = wide_rows(p);
+    if (p.out_bf16) return vec ? launch_tile_cut<BM, BN, PER_CU, true, true>(stream, p) : launch_tile_cut<BM, BN, PER_CU, true, false>(stream, p);
+    return vec ? launch_tile_cut<BM, BN, PER_CU, false, true>(stream, p) : launch_tile_cut<BM, BN, PER_CU, false, false>(stream, p);
 }
 
 }  // namespace
