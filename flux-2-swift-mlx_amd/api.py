@@ -108,6 +108,7 @@ class Context:
         self.device = torch.device("cuda", device)
         torch.cuda.set_device(self.device)
         self.stream = torch.cuda.Stream(device=self.device)
+        self._raw_stream = self.stream.cuda_stream
         h = C.c_void_p()
         check(lib().flux2mi_ctx_create(device, C.c_void_p(self.stream.cuda_stream), C.byref(h)))
         self.handle = h
@@ -115,14 +116,12 @@ class Context:
 
     # stream ordering against torch's current stream (no host sync; nothing to order inside `with torch.cuda.stream(ctx.stream)`)
     def _enter(self):
-        current = torch.cuda.current_stream(self.device)
-        if current.cuda_stream != self.stream.cuda_stream:
-            self.stream.wait_stream(current)
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._raw_stream:
+            self.stream.wait_stream(torch.cuda.current_stream(self.device))
 
     def _exit(self):
-        current = torch.cuda.current_stream(self.device)
-        if current.cuda_stream != self.stream.cuda_stream:
-            current.wait_stream(self.stream)
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._raw_stream:
+            torch.cuda.current_stream(self.device).wait_stream(self.stream)
 
     def sync(self):
         check(lib().flux2mi_ctx_sync(self.handle))
@@ -542,11 +541,14 @@ class Context:
     def _mxfp4(self, m: MXFP4, name: str) -> MXFP4:
         codes, scales, cols = m
         pad = -(-int(cols) // 128) * 128
-        for t, what, width in ((codes, "codes", pad // 2), (scales, "scales", pad // 32)):
-            if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.uint8:
+        for t, what in ((codes, "codes"), (scales, "scales")):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.device != self.device:
                 raise Flux2Error(L.ERR_INVALID_ARG, f"{name}.{what} must be a torch.uint8 tensor on {self.device}")
-            if cols < 1 or t.dim() != 2 or t.shape != (codes.shape[0], width):
-                raise Flux2Error(L.ERR_SHAPE, f"{name}.{what} must have shape ({codes.shape[0]}, {width}) for {cols} columns, got {tuple(t.shape)}")
+        if cols < 1 or codes.dim() != 2 or codes.shape[1] * 2 != pad or scales.shape != (codes.shape[0], pad // 32):
+            raise Flux2Error(L.ERR_SHAPE, f"{name}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} for {cols} columns: "
+                                          f"[rows, {pad // 2}] and [rows, {pad // 32}] are wanted")
+        if codes.is_contiguous() and scales.is_contiguous():
+            return m
         return MXFP4(codes.contiguous(), scales.contiguous(), int(cols))
 
     def op_quantize_mxfp4(self, x: torch.Tensor) -> MXFP4:

@@ -67,16 +67,24 @@ __device__ __forceinline__ bf16x8 load_a8(const uint16_t* row, int k, int K) {
     return __builtin_bit_cast(bf16x8, u);
 }
 
-// ---------------------------------------------------------------------------------------------- a tile per workgroup, K split over its waves
-// 16 MT rows x 16 NT columns; the four waves take the 128-value steps in turn and their sums are added in wave order through LDS.
-template <bool A4, bool AVEC, bool VEC, int MT, int NT>
-__global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n) {
-    __shared__ f32x4 part[4][MT * NT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+// ---------------------------------------------------------------------------------------------- few rows: K split over the waves of a workgroup
+// 16 MT rows x 16 NT columns per workgroup; its WAVES waves take the 128-value steps in turn (so that together they read whole lines of W) and
+// their sums are added in wave order through LDS.  Bound by reading W: operands go straight from memory to registers, U steps of a wave at a
+// time, and the next U are requested before the current ones are used.
+template <int MT, int NT>
+struct RowsStep {
+    u32x4 w[NT], a[MT];
+    uint32_t sw[NT], sa[MT];
+};
+
+template <bool VEC, int MT, int NT, int U, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n) {
+    __shared__ f32x4 part[WAVES][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int n0 = (int)(blockIdx.x % tiles_n) * 16 * NT, m0 = (int)(blockIdx.x / tiles_n) * 16 * MT;
     const int64_t row_bytes = (int64_t)p.steps * 64, row_scales = (int64_t)p.steps * 4;
+    const int steps = p.steps;
     const uint8_t *wq[NT], *ws[NT], *aq[MT], *as[MT];
-    const uint16_t* ab[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {   // rows behind the last one: its copy, never stored
         const int64_t n = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
@@ -86,49 +94,54 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int t
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t m = m0 + 16 * i + r < p.M ? m0 + 16 * i + r : p.M - 1;
-        if constexpr (A4) {
-            aq[i] = reinterpret_cast<const uint8_t*>(p.a) + m * row_bytes + g * 16;
-            as[i] = p.a_scales + m * row_scales + g;
-        } else ab[i] = reinterpret_cast<const uint16_t*>(p.a) + m * p.lda;
+        aq[i] = reinterpret_cast<const uint8_t*>(p.a) + m * row_bytes + g * 16;
+        as[i] = p.a_scales + m * row_scales + g;
     }
+    auto load = [&](int s, RowsStep<MT, NT>& x) {
+        if (s >= steps) return;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            x.w[j] = *reinterpret_cast<const u32x4*>(wq[j] + (int64_t)s * 64);
+            x.sw[j] = ws[j][(int64_t)s * 4];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            x.a[i] = *reinterpret_cast<const u32x4*>(aq[i] + (int64_t)s * 64);
+            x.sa[i] = as[i][(int64_t)s * 4];
+        }
+    };
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = wave; s < p.steps; s += 4) {
-        u32x4 w[NT];
-        uint32_t sw[NT];
+    auto use = [&](int s, const RowsStep<MT, NT>& x) {
+        if (s >= steps) return;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            w[j] = *reinterpret_cast<const u32x4*>(wq[j] + (int64_t)s * 64);
-            sw[j] = ws[j][(int64_t)s * 4];
-        }
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            if constexpr (A4) {
-                const u32x4 a = *reinterpret_cast<const u32x4*>(aq[i] + (int64_t)s * 64);
-                const uint32_t sa = as[i][(int64_t)s * 4];
+            for (int j = 0; j < NT; ++j) acc[j][i] = mfma_fp4(x.w[j], x.a[i], acc[j][i], x.sw[j], x.sa[i]);
+    };
+    RowsStep<MT, NT> cur[U], next[U];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][i] = mfma_fp4(w[j], a, acc[j][i], sw[j], sa);
-            } else {
+    for (int u = 0; u < U; ++u) load(wave + u * WAVES, cur[u]);
+    for (int s = wave; s < steps; s += U * WAVES) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const bf16x8 a = load_a8<AVEC>(ab[i], s * 128 + g * 32 + q * 8, p.K);
+        for (int u = 0; u < U; ++u) load(s + (U + u) * WAVES, next[u]);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(w[j][q], __builtin_bit_cast(float, sw[j] << 23)), a, acc[j][i], 0, 0, 0);
-                }
-            }
-        }
+        for (int u = 0; u < U; ++u) use(s + u * WAVES, cur[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur[u] = next[u];
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) part[wave][j * MT + i][lane] = acc[j][i];
     __syncthreads();
-    for (int t = wave; t < MT * NT; t += 4) {
-        const f32x4 v = part[0][t][lane] + part[1][t][lane] + part[2][t][lane] + part[3][t][lane];
+    for (int t = wave; t < MT * NT; t += WAVES) {
+        f32x4 v = part[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += part[w][t][lane];
         store4<VEC>(p, m0 + 16 * (t % MT) + r, n0 + 16 * (t / MT) + 4 * g, v);
     }
 }
@@ -559,25 +572,346 @@ bool wide_rows(const Mxfp4Gemm& p) {
     const int cols = p.out_bf16 ? 8 : 4;
     return p.N % cols == 0 && ok(p.out, p.ld_out, cols) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
 }
+// ---------------------------------------------------------------------------------------------- the same with A in bf16
+// A is shared by every wave of a workgroup and comes once per workgroup through LDS, `chunk` steps of all its rows at a time (chunk % WAVES == 0, so
+// that a wave's steps wave, wave + WAVES, ... fall into the chunks alike); W and its scales stream through registers across the chunks.
+// Read by every wave for itself, A costs four loads per step against one of W: the vector-memory path, not HBM, is then the bound.
+template <bool AVEC, bool VEC, int MT, int NT, int U, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n, int chunk) {
+    extern __shared__ __align__(16) uint8_t smem[];   // A: [rows][chunk * 256 + 16] bytes; then the partial sums [WAVES][MT * NT][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int n0 = (int)(blockIdx.x % tiles_n) * 16 * NT, m0 = (int)(blockIdx.x / tiles_n) * 16 * MT;
+    const int64_t row_bytes = (int64_t)p.steps * 64, row_scales = (int64_t)p.steps * 4;
+    const int steps = p.steps, rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT, pitch = chunk * 256 + 16;
+    const uint8_t *wq[NT], *ws[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {   // rows behind the last one: its copy, never stored
+        const int64_t n = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
+        wq[j] = p.w + n * row_bytes + g * 16;
+        ws[j] = p.w_scales + n * row_scales + g;
+    }
+    struct Step { u32x4 w[NT]; uint32_t s[NT]; };
+    auto load = [&](int s, Step& x) {
+        if (s >= steps) return;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            x.w[j] = *reinterpret_cast<const u32x4*>(wq[j] + (int64_t)s * 64);
+            x.s[j] = ws[j][(int64_t)s * 4];
+        }
+    };
+    const uint16_t* a = reinterpret_cast<const uint16_t*>(p.a);
+    auto stage = [&](int first) {   // steps first ... first + chunk - 1 of A; columns >= K are zero
+        const int pieces = chunk * 16;   // of a row, 8 values each
+        for (int at = threadIdx.x; at < rows * pieces; at += 64 * WAVES) {
+            const int row = at / pieces, c = at - row * pieces, k = first * 128 + c * 8;
+            if (k < steps * 128) *reinterpret_cast<bf16x8*>(smem + row * pitch + c * 16) = load_a8<AVEC>(a + (int64_t)(m0 + row) * p.lda, k, p.K);
+        }
+    };
+    const uint8_t* arow[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) arow[i] = smem + (16 * i + r < rows ? 16 * i + r : rows - 1) * pitch + g * 64;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto use = [&](int s, int first, const Step& x) {
+        if (s >= steps) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            bf16x8 b[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) b[i] = *reinterpret_cast<const bf16x8*>(arow[i] + (s - first) * 256 + q * 16);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const bf16x8 w = codes_to_bf16(x.w[j][q], __builtin_bit_cast(float, x.s[j] << 23));
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, b[i], acc[j][i], 0, 0, 0);
+            }
+        }
+    };
+    Step cur[U], next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(wave + u * WAVES, cur[u]);
+    for (int first = 0; first < steps; first += chunk) {
+        if (first) __syncthreads();   // the previous chunk has been read
+        stage(first);
+        __syncthreads();
+        const int end = first + chunk < steps ? first + chunk : steps;
+        for (int s = first + wave; s < end; s += U * WAVES) {   // (a wave without a step left in the chunk has none later either)
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(s + (U + u) * WAVES, next[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) use(s + u * WAVES, first, cur[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) cur[u] = next[u];
+        }
+    }
+    __syncthreads();
+    f32x4* part = reinterpret_cast<f32x4*>(smem);   // [WAVES][MT * NT][64]
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) part[(wave * MT * NT + j * MT + i) * 64 + lane] = acc[j][i];
+    __syncthreads();
+    for (int t = wave; t < MT * NT; t += WAVES) {
+        f32x4 v = part[t * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += part[(w * MT * NT + t) * 64 + lane];
+        store4<VEC>(p, m0 + 16 * (t % MT) + r, n0 + 16 * (t / MT) + 4 * g, v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- tiles staged through LDS (bf16 x MXFP4)
+// BM x BN outputs per workgroup of WM x WN waves.  A stage is one 128-k step: 256 bytes of every A row, 64 bytes of codes and 4 scale bytes of every
+// W row, all by LDS-DMA into a ring of STAGES buffers; STAGES - 1 of them are requested ahead and the wait is counted, so the stream is never drained.
+// W's codes become bf16 in registers (4 conversions per 8 values, used by MT MFMAs), a lane's scale is one byte of the row's four.
+// Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7, W: by (row / 2) & 3) so that fragment reads meet no bank conflicts.
+// A of any alignment (AVEC false) passes through registers instead, a stage ahead; columns >= K are zeroed where the last stage is read or staged.
+__device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
+    u32x4 u = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t w = u[d];
+        u[d] = keep >= 2 * d + 2 ? w : keep == 2 * d + 1 ? w & 0xffffu : 0u;
+    }
+    return __builtin_bit_cast(bf16x8, u);
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool AVEC, bool BF16, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN * KG) void bf16_mxfp4_gemm_tile_kernel(Mxfp4Gemm p, int tiles_m, int tiles_n, int band) {
+    constexpr int WAVES = WM * WN * KG, MT = BM / (16 * WM), NT = BN / (16 * WN);
+    constexpr int A_BYTES = BM * 256, W_BYTES = BN * 64, STAGE = KG * (A_BYTES + W_BYTES);
+    constexpr bool PAIR = KG % 2 == 0;   // W's codes of two steps together: whole 128-byte lines
+    constexpr int PA = BM / 4, PW = BN / 16, CNT_A = KG * PA / WAVES, CNT_W = KG * PW / WAVES, CNT = (AVEC ? CNT_A : 0) + CNT_W;   // pieces of a step; per wave and stage
+    static_assert(CNT_A * WAVES == KG * PA && CNT_W * WAVES == KG * PW, "whole pieces");
+    constexpr int TPG = 4 / KG, AHEAD = (STAGES - 1 + TPG - 1) / TPG, SBUF = AHEAD + 1;   // stages per scale group; groups requested ahead; their buffers
+    extern __shared__ __align__(1024) uint8_t smem[];   // [STAGES]{[KG] A, [KG] W}, [SBUF][BN][16] scales
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % WM, wn = wave / WM % WN;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, band, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN, steps = p.steps, stages = (steps + KG - 1) / KG, whole = (steps - 1) / KG;   // stages in front of `whole` lie inside K
+    const uint32_t row_bytes = (uint32_t)steps * 64, row_scales = (uint32_t)steps * 4, a_bytes = (uint32_t)p.lda * 2;
+    const uint8_t* abase = reinterpret_cast<const uint8_t*>(p.a) + (int64_t)m0 * p.lda * 2;
+    const uint8_t* wbase = p.w + (int64_t)n0 * row_bytes;
+    const uint8_t* sbase = p.w_scales + (int64_t)n0 * row_scales;
+    const int last_w = p.N - 1 - n0, last_a = p.M - 1 - m0;   // rows behind the last one: its copy, never stored
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+
+    // piece k of this wave's A (W) pieces of a stage: step `first + k` / PA (PW) of the stage
+    auto a_row = [&](int k) { const int row = (wave * CNT_A + k) % PA * 4 + (lane >> 4); return row; };
+    auto a_chunk = [&](int k) { return (lane & 8) | ((lane & 7) ^ (a_row(k) & 7)); };
+    uint32_t va[CNT_A], vw[CNT_W], vs[(PW + WAVES - 1) / WAVES];
+#pragma unroll
+    for (int k = 0; k < CNT_A; ++k) {
+        const int row = a_row(k), step = (wave * CNT_A + k) / PA;
+        va[k] = (uint32_t)(row < last_a ? row : last_a) * a_bytes + a_chunk(k) * 16 + step * 256;
+    }
+    // W: pieces of 16 rows x one step, or 8 rows x two
+    auto w_row = [&](int k) { const int i = wave * CNT_W + k; return PAIR ? i % (BN / 8) * 8 + (lane >> 3) : i % PW * 16 + (lane >> 2); };
+    auto w_chunk = [&](int k) { return PAIR ? (lane & 7) ^ (w_row(k) & 7) : (lane & 3) ^ (w_row(k) >> 1 & 3); };
+    auto w_step = [&](int k) { const int i = wave * CNT_W + k; return PAIR ? i / (BN / 8) * 2 + (w_chunk(k) >> 2) : i / PW; };
+#pragma unroll
+    for (int k = 0; k < CNT_W; ++k) vw[k] = (uint32_t)(w_row(k) < last_w ? w_row(k) : last_w) * row_bytes + w_step(k) * 64 + (w_chunk(k) & 3) * 16;
+#pragma unroll
+    for (int k = 0; k < (PW + WAVES - 1) / WAVES; ++k) {
+        const int row = (wave + WAVES * k) * 16 + (lane >> 2);
+        vs[k] = (uint32_t)(row < last_w ? row : last_w) * row_scales;
+    }
+    // Four steps' scales at a time (what the vector-memory path counts is lines, and a row's line is touched once for them).
+    auto issue_scales = [&](int group) {
+        const int t = group * 4 + (lane & 3), step = t < steps ? t : steps - 1;
+#pragma unroll
+        for (int k = 0; k < (PW + WAVES - 1) / WAVES; ++k)
+            if (wave + WAVES * k < PW) dma4(vs[k] + step * 4, sbase, lds0 + STAGES * STAGE + (uint32_t)(group % SBUF) * (BN * 16) + (wave + WAVES * k) * 256);
+    };
+    auto issue = [&](int t, int buf) {   // stage t; behind the end the last one again, so that every stage counts alike
+        const uint32_t at = lds0 + (uint32_t)buf * STAGE;
+        auto a_lds = [&](int k) { const int i = wave * CNT_A + k; return at + i * 1024; };
+        auto w_lds = [&](int k) { const int i = wave * CNT_W + k; return at + KG * A_BYTES + i * 1024; };
+        if (t < whole) {
+            if constexpr (AVEC) {
+#pragma unroll
+                for (int k = 0; k < CNT_A; ++k) dma16(va[k], abase + (int64_t)t * (KG * 256), a_lds(k));
+            }
+#pragma unroll
+            for (int k = 0; k < CNT_W; ++k) dma16(vw[k], wbase + (int64_t)t * (KG * 64), w_lds(k));
+        } else {   // steps and chunks behind K are fetched from the last ones (AVEC: K % 8 == 0); nothing uses them
+            const int last = steps - 1, first = whole * KG;
+            const uint32_t end = (uint32_t)p.K * 2 - 16;
+            if constexpr (AVEC) {
+#pragma unroll
+                for (int k = 0; k < CNT_A; ++k) {
+                    const int s = (wave * CNT_A + k) / PA, step = first + s < last ? first + s : last, row = a_row(k);
+                    const uint32_t col = (uint32_t)step * 256 + a_chunk(k) * 16;
+                    dma16((uint32_t)(row < last_a ? row : last_a) * a_bytes + (col < end ? col : end), abase, a_lds(k));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < CNT_W; ++k) {
+                const int s = w_step(k), step = first + s < last ? first + s : last;
+                dma16(vw[k] + (uint32_t)(step - s) * 64, wbase, w_lds(k));
+            }
+        }
+    };
+    // AVEC false: A through registers, chunk `tid + 64 WAVES c` of the stage's KG BM rows of 16
+    constexpr int AC = KG * BM * 16 / (64 * WAVES);
+    static_assert(AC * 64 * WAVES == KG * BM * 16, "whole chunks");
+    u32x4 areg[AVEC ? 1 : AC];
+    auto fetch_a = [&](int t) {
+        if constexpr (!AVEC) {
+#pragma unroll
+            for (int c = 0; c < AC; ++c) {
+                const int at = threadIdx.x + 64 * WAVES * c, row = (at >> 4) % BM, step = t * KG + (at >> 4) / BM, k = step * 128 + (at & 15) * 8;
+                areg[c] = u32x4{0, 0, 0, 0};
+                if (k < p.K) areg[c] = __builtin_bit_cast(u32x4, load_a8<false>(reinterpret_cast<const uint16_t*>(abase + (int64_t)(row < last_a ? row : last_a) * a_bytes), k, p.K));
+            }
+        }
+    };
+    auto put_a = [&](int buf) {
+        if constexpr (!AVEC) {
+#pragma unroll
+            for (int c = 0; c < AC; ++c) {
+                const int at = threadIdx.x + 64 * WAVES * c, row = (at >> 4) % BM, s = (at >> 4) / BM, ch = at & 15;
+                *reinterpret_cast<u32x4*>(smem + buf * STAGE + s * A_BYTES + row * 256 + ((ch & 8) | ((ch & 7) ^ (row & 7))) * 16) = areg[c];
+            }
+        }
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int s, int buf, auto last) {   // step s, this wave's of the stage in `buf`
+        const uint8_t* arow = smem + buf * STAGE + kg * A_BYTES + (wm * MT * 16 + r) * 256;
+        const uint8_t* wrow = smem + buf * STAGE + KG * A_BYTES + (PAIR ? kg / 2 * (BN * 128) + (wn * NT * 16 + r) * 128 + (((kg & 1) * 4 + g) ^ (r & 7)) * 16
+                                                                       : kg * W_BYTES + (wn * NT * 16 + r) * 64 + (g ^ (r >> 1 & 3)) * 16);
+        const uint8_t* srow = smem + STAGES * STAGE + (s >> 2) % SBUF * (BN * 16) + (wn * NT * 16 + r) * 16 + (s & 3) * 4 + g;
+        u32x4 w[NT];
+        float sc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            w[j] = *reinterpret_cast<const u32x4*>(wrow + j * (PAIR ? 2048 : 1024));
+            sc[j] = __builtin_bit_cast(float, (uint32_t)srow[j * 256] << 23);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            bf16x8 a[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int c = 4 * g + q;   // (row & 7 = r & 7 in every 16-row block)
+                a[i] = *reinterpret_cast<const bf16x8*>(arow + i * 4096 + ((c & 8) | ((c & 7) ^ (r & 7))) * 16);
+                if constexpr (AVEC && decltype(last)::value) a[i] = zero_from(a[i], p.K - s * 128 - c * 8);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint32_t code = w[j][q];
+                const bf16x8 b = codes_to_bf16(code, sc[j]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[i], acc[j][i], 0, 0, 0);
+            }
+        }
+    };
+    fetch_a(0);
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) issue_scales(q);
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) issue(t, t);
+    put_a(0);
+    fetch_a(1);
+    int buf = 0, before = STAGES - 1;   // t % STAGES, (t - 1) % STAGES
+    auto turn = [&](int t, auto last) {
+        constexpr int FLY = (STAGES - 2) * CNT;   // (a wave's scale pieces come on top: it then waits for that much more, never for less)
+        static_assert(FLY < 64, "vmcnt");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (FLY & 15) | (FLY >> 4 << 14));   // stage t has landed; lgkmcnt 0
+        asm volatile("s_barrier" ::: "memory");
+        if (t % TPG == 0) issue_scales(t / TPG + AHEAD);
+        issue(t + STAGES - 1, before);   // into the buffer of stage t - 1, which everybody has left
+        const int after = buf + 1 < STAGES ? buf + 1 : 0;
+        put_a(after);
+        fetch_a(t + 2);
+        if constexpr (decltype(last)::value) {
+            if (t * KG + kg < steps - 1) compute(t * KG + kg, buf, std::false_type{});
+            else if (t * KG + kg == steps - 1) compute(steps - 1, buf, std::true_type{});
+        } else compute(t * KG + kg, buf, std::false_type{});
+        before = buf;
+        buf = after;
+    };
+    for (int t = 0; t + 1 < stages; ++t) turn(t, std::false_type{});
+    turn(stages - 1, std::true_type{});
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if constexpr (KG > 1) {   // the k groups' sums, added in their order
+        f32x4* part = reinterpret_cast<f32x4*>(smem);
+        if (kg > 0) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) part[((wave - WM * WN) * NT * MT + j * MT + i) * 64 + lane] = acc[j][i];
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int h = 0; h < KG - 1; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[j][i] += part[((wave + h * WM * WN) * NT * MT + j * MT + i) * 64 + lane];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+    }
+    if constexpr (NT >= 4) {
+        uint8_t* mine = smem + wave * 2 * store_slot_bytes<MT, NT, BF16>();
+        if (p.bias || p.gate) store_tile<MT, NT, BF16, VEC, true>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+        else store_tile<MT, NT, BF16, VEC, false>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) store4<VEC>(p, m0 + (wm * MT + i) * 16 + r, n0 + (wn * NT + j) * 16 + 4 * g, acc[j][i]);
+    }
+}
+
+constexpr int64_t MAX_TILES = 1 << 22;   // x 512 threads: below 2^32 in a launch
+
 bool four_columns(const Mxfp4Gemm& p) {
     auto ok = [](const void* q, int64_t ld, int esz) { return !q || (reinterpret_cast<uintptr_t>(q) % (4 * esz) == 0 && ld % 4 == 0); };
     return p.N % 4 == 0 && ok(p.out, p.ld_out, p.out_bf16 ? 2 : 4) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
 }
 
-template <bool A4, bool AVEC, int MT, int NT>
+template <int MT, int NT, int U, int WAVES>
 int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
-    if (tn * tm >= (1 << 24)) return 1;
-    const dim3 grid((unsigned)(tn * tm)), block(256);
-    if (four_columns(p)) mxfp4_gemm_rows_kernel<A4, AVEC, true, MT, NT><<<grid, block, 0, stream>>>(p, (int)tn);
-    else mxfp4_gemm_rows_kernel<A4, AVEC, false, MT, NT><<<grid, block, 0, stream>>>(p, (int)tn);
+    if (tn * tm >= MAX_TILES) return 1;
+    const dim3 grid((unsigned)(tn * tm)), block(64 * WAVES);
+    if (four_columns(p)) mxfp4_gemm_rows_kernel<true, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
+    else mxfp4_gemm_rows_kernel<false, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
+template <bool AVEC, int MT, int NT, int U, int WAVES>
+int launch_bf16_rows(hipStream_t stream, const Mxfp4Gemm& p) {
+    const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
+    if (tn * tm >= MAX_TILES) return 1;
+    const int rows = p.M < 16 * MT ? p.M : 16 * MT, unit = WAVES * U;
+    int chunk = 65536 / (rows * 256) / unit * unit;                    // A's part of LDS: 64 KB
+    if (chunk < unit) chunk = unit;
+    const int all = (p.steps + unit - 1) / unit * unit;
+    if (chunk > all) chunk = all;
+    const int lds_a = rows * (chunk * 256 + 16), lds_sums = WAVES * MT * NT * 1024, lds = lds_a > lds_sums ? lds_a : lds_sums;
+    const dim3 grid((unsigned)(tn * tm)), block(64 * WAVES);
+    const bool vec = four_columns(p);
+    const auto fn = vec ? bf16_mxfp4_gemm_rows_kernel<AVEC, true, MT, NT, U, WAVES> : bf16_mxfp4_gemm_rows_kernel<AVEC, false, MT, NT, U, WAVES>;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return 2;
+    fn<<<grid, block, lds, stream>>>(p, (int)tn, chunk);
+    return hipGetLastError() == hipSuccess ? 0 : 2;
+}
 template <int BM, int BN, int PER_CU, bool BF16, bool VEC, int CUT>
 int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tn * tm >= (1 << 24)) return 1;
+    if (tn * tm >= MAX_TILES) return 1;
     constexpr int LDS = (BM + BN) * (2 * 128 + 3 * 16);
     const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, CUT, PER_CU>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
@@ -597,14 +931,72 @@ int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
     return vec ? launch_tile_cut<BM, BN, PER_CU, false, true>(stream, p) : launch_tile_cut<BM, BN, PER_CU, false, false>(stream, p);
 }
 
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool AVEC, bool BF16, bool VEC>
+int launch_bf16_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
+    const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+    if (tn * tm >= MAX_TILES) return 1;
+    constexpr int NT = BN / (16 * WN), MT = BM / (16 * WM), TPG = 4 / KG, SBUF = (STAGES - 1 + TPG - 1) / TPG + 1;
+    constexpr int RING = STAGES * KG * (BM * 256 + BN * 64) + SBUF * BN * 16, EPI = NT >= 4 ? WM * WN * 2 * store_slot_bytes<MT, NT, BF16>() : 0;
+    constexpr int SUMS = (KG - 1) * WM * WN * NT * MT * 1024, LDS = RING > EPI ? (RING > SUMS ? RING : SUMS) : (EPI > SUMS ? EPI : SUMS);
+    static_assert(LDS <= 163840, "160 KB");
+    const auto fn = bf16_mxfp4_gemm_tile_kernel<BM, BN, WM, WN, KG, STAGES, AVEC, BF16, VEC>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
+    fn<<<dim3((unsigned)(tn * tm)), dim3(64 * WM * WN * KG), LDS, stream>>>(p, (int)tm, (int)tn, 6);
+    return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool AVEC>
+int launch_bf16_tile(hipStream_t stream, const Mxfp4Gemm& p) {
+    const bool vec = BN / WN >= 64 ? wide_rows(p) : four_columns(p);
+    if (p.out_bf16) return vec ? launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, true, true>(stream, p) : launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, true, false>(stream, p);
+    return vec ? launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, false, true>(stream, p) : launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, false, false>(stream, p);
+}
+
+// Tile of A in bf16: the launch's rounds (256 CUs, a workgroup each) x what a 128-k step of a full round takes, us, measured at 64 ... 4608 rows x 4096 /
+// 12288 columns.  A larger tile does more per step and byte, a smaller one fills the chip at fewer rows.
+struct Bf16Tile { int bm, bn; double us; };
+constexpr Bf16Tile BF16_TILES[] = {{32, 128, 0.35}, {64, 128, 0.56}, {64, 256, 0.97}, {128, 256, 1.70}};
+int pick_bf16_tile(const Mxfp4Gemm& p) {
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t tiles = (int64_t)((p.M + BF16_TILES[i].bm - 1) / BF16_TILES[i].bm) * ((p.N + BF16_TILES[i].bn - 1) / BF16_TILES[i].bn);
+        const double t = (double)((tiles + 255) / 256) * BF16_TILES[i].us;
+        if (t < least) { least = t; best = i; }
+    }
+    return best;
+}
+
+// 256 x 256 tiles, one per CU, or 128 x 128, two: measured, a group of 512 k of a round of 256 (512) tiles takes 4.4 (2.7) us, of up to 256 small ones 1.5.
+bool large_tiles(const Mxfp4Gemm& p) {
+    const int64_t big = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256), small = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128), rest = small % 512;
+    return (double)((big + 255) / 256) * 4.4 < (double)(small / 512) * 2.7 + (rest == 0 ? 0.0 : rest <= 256 ? 1.5 : 2.7);
+}
+
 }  // namespace
 
 int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
-    if (p.a_scales && p.K < (1 << 24)) {
-        if (p.M > 128 && (int64_t)p.M * p.N >= (int64_t)256 * 256 * 200) return launch_tile<256, 256, 1>(stream, p);
-        if (p.M > 32) return launch_tile<128, 128, 2>(stream, p);
+    const bool offsets32 = p.K < (1 << 24) && p.lda < (1 << 24);   // row offsets inside a tile fit 32 bits
+    if (p.a_scales) {
+        // up to 16 rows W is read once by 16-column workgroups: 4096 x 12288 8.8 us (one row); its 32 tiles of 128 columns would take 32.  Up to 64
+        // rows the tiles are faster as soon as there are 64 of them (32 x 12288 x 4096: 13.5 us against 18.1).
+        if (p.M <= 16 || !offsets32) return launch_rows<1, 1, 4, 4>(stream, p);
+        if (p.M <= 64 && p.N < 64 * 128) return launch_rows<2, 1, 4, 8>(stream, p);
+        return large_tiles(p) ? launch_tile<256, 256, 1>(stream, p) : launch_tile<128, 128, 2>(stream, p);
     }
-    if (p.a_scales) return launch_rows<true, false, 2, 2>(stream, p);
-    const bool avec = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
-    return avec ? launch_rows<false, true, 2, 2>(stream, p) : launch_rows<false, false, 2, 2>(stream, p);
+    const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
+    // few rows: A whole in LDS (1 x 19456 x 2560 8.5 us, 16-row tiles 11; at 16 rows 23.7 against 8.7)
+    if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true, 1, 1, 2, 8>(stream, p) : launch_bf16_rows<false, 1, 1, 2, 8>(stream, p);
+    const bool dma = aligned && p.K % 8 == 0;   // A by DMA, or through registers
+    if (p.M <= 32) {
+        // 16-row tiles; 64 columns as soon as these fill the chip, else 32 and four k groups (23 x 5120 x 5120: 9.0 us against 9.9; 16 x 19456 x 2560: 9.8, 8.7)
+        const bool wide = (int64_t)((p.M + 15) / 16) * ((p.N + 63) / 64) >= 256;
+        if (wide) return dma ? launch_bf16_tile<16, 64, 1, 4, 2, 3, true>(stream, p) : launch_bf16_tile<16, 64, 1, 4, 2, 3, false>(stream, p);
+        return dma ? launch_bf16_tile<16, 32, 1, 2, 4, 3, true>(stream, p) : launch_bf16_tile<16, 32, 1, 2, 4, 3, false>(stream, p);
+    }
+    const int tile = pick_bf16_tile(p);
+    if (!dma) return tile == 3 ? launch_bf16_tile<128, 256, 2, 4, 1, 3, false>(stream, p) : launch_bf16_tile<64, 128, 1, 4, 2, 3, false>(stream, p);
+    if (tile == 0) return launch_bf16_tile<32, 128, 1, 4, 2, 3, true>(stream, p);
+    if (tile == 1) return launch_bf16_tile<64, 128, 1, 4, 2, 3, true>(stream, p);
+    if (tile == 2) return launch_bf16_tile<64, 256, 1, 4, 2, 2, true>(stream, p);
+    return launch_bf16_tile<128, 256, 2, 4, 1, 3, true>(stream, p);
 }
