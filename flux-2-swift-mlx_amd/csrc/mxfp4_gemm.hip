@@ -56,14 +56,25 @@ __device__ __forceinline__ void store4(const Mxfp4Gemm& p, int m, int n, f32x4 v
     }
 }
 
-// 8 values of a bf16 row from column k on; columns >= K (the padding of W's last step) are zero
+// 8 values of a bf16 row from column k on; columns >= K (the padding of W's last step) are zero.  AVEC: 16-byte aligned; otherwise the row may start
+// anywhere: the 8 values' dwords, shifted by half a dword where they are odd (no dword without one of the values is read).
 template <bool AVEC>
 __device__ __forceinline__ bf16x8 load_a8(const uint16_t* row, int k, int K) {
-    if (AVEC && k + 8 <= K) return *reinterpret_cast<const bf16x8*>(row + k);
+    typedef u32x4 __attribute__((aligned(4))) u32x4_dword;
     u32x4 u = {0, 0, 0, 0};
+    if (k + 8 <= K) {
+        if constexpr (AVEC) return *reinterpret_cast<const bf16x8*>(row + k);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row + k);
+        const uint32_t shift = (at & 2) * 8;
+        const u32x4 d = *reinterpret_cast<const u32x4_dword*>(at & ~(uintptr_t)3);
+        const uint32_t e = *reinterpret_cast<const uint32_t*>((at & ~(uintptr_t)3) + (shift ? 16 : 12));
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (k + j < K) u[j >> 1] |= (uint32_t)row[k + j] << (16 * (j & 1));
+        for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_alignbit(j < 3 ? d[j < 3 ? j + 1 : 3] : e, d[j], shift);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (k + j < K) u[j >> 1] |= (uint32_t)row[k + j] << (16 * (j & 1));
+    }
     return __builtin_bit_cast(bf16x8, u);
 }
 
@@ -667,7 +678,8 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
 // W row, all by LDS-DMA into a ring of STAGES buffers; STAGES - 1 of them are requested ahead and the wait is counted, so the stream is never drained.
 // W's codes become bf16 in registers (4 conversions per 8 values, used by MT MFMAs), a lane's scale is one byte of the row's four.
 // Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7, W: by (row / 2) & 3) so that fragment reads meet no bank conflicts.
-// A of any alignment (AVEC false) passes through registers instead, a stage ahead; columns >= K are zeroed where the last stage is read or staged.
+// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead.  Columns >= K are zeroed where
+// the last stage is read or staged.
 __device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
     u32x4 u = __builtin_bit_cast(u32x4, v);
 #pragma unroll
@@ -737,7 +749,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void bf16_mxfp4_gemm_tile_kernel
             }
 #pragma unroll
             for (int k = 0; k < CNT_W; ++k) dma16(vw[k], wbase + (int64_t)t * (KG * 64), w_lds(k));
-        } else {   // steps and chunks behind K are fetched from the last ones (AVEC: K % 8 == 0); nothing uses them
+        } else {   // steps and chunks behind K are fetched from the last ones: a row's last 16 bytes, also for a chunk that K cuts
             const int last = steps - 1, first = whole * KG;
             const uint32_t end = (uint32_t)p.K * 2 - 16;
             if constexpr (AVEC) {
@@ -802,7 +814,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void bf16_mxfp4_gemm_tile_kernel
             for (int i = 0; i < MT; ++i) {
                 const int c = 4 * g + q;   // (row & 7 = r & 7 in every 16-row block)
                 a[i] = *reinterpret_cast<const bf16x8*>(arow + i * 4096 + ((c & 8) | ((c & 7) ^ (r & 7))) * 16);
-                if constexpr (AVEC && decltype(last)::value) a[i] = zero_from(a[i], p.K - s * 128 - c * 8);
+                if constexpr (AVEC && decltype(last)::value) {
+                    const int keep = p.K - s * 128 - c * 8;   // (even)
+                    if (keep > 0 && keep < 8) {               // fetched 8 - keep values early
+                        const u32x4 u = __builtin_bit_cast(u32x4, a[i]);
+                        a[i] = __builtin_bit_cast(bf16x8, keep == 6 ? u32x4{u[1], u[2], u[3], 0} : keep == 4 ? u32x4{u[2], u[3], 0, 0} : u32x4{u[3], 0, 0, 0});
+                    }
+                    a[i] = zero_from(a[i], keep);
+                }
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -827,10 +846,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void bf16_mxfp4_gemm_tile_kernel
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0070 | (FLY & 15) | (FLY >> 4 << 14));   // stage t has landed; lgkmcnt 0
         asm volatile("s_barrier" ::: "memory");
+        const int after = buf + 1 < STAGES ? buf + 1 : 0;
+        put_a(after);                    // (in front of the requests: its registers' wait would take them along)
         if (t % TPG == 0) issue_scales(t / TPG + AHEAD);
         issue(t + STAGES - 1, before);   // into the buffer of stage t - 1, which everybody has left
-        const int after = buf + 1 < STAGES ? buf + 1 : 0;
-        put_a(after);
         fetch_a(t + 2);
         if constexpr (decltype(last)::value) {
             if (t * KG + kg < steps - 1) compute(t * KG + kg, buf, std::false_type{});
@@ -986,7 +1005,7 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
     const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
     // few rows: A whole in LDS (1 x 19456 x 2560 8.5 us, 16-row tiles 11; at 16 rows 23.7 against 8.7)
     if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true, 1, 1, 2, 8>(stream, p) : launch_bf16_rows<false, 1, 1, 2, 8>(stream, p);
-    const bool dma = aligned && p.K % 8 == 0;   // A by DMA, or through registers
+    const bool dma = reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && p.lda % 2 == 0 && p.K % 2 == 0 && p.K >= 8;   // A by DMA, or through registers
     if (p.M <= 32) {
         // 16-row tiles; 64 columns as soon as these fill the chip, else 32 and four k groups (23 x 5120 x 5120: 9.0 us against 9.9; 16 x 19456 x 2560: 9.8, 8.7)
         const bool wide = (int64_t)((p.M + 15) / 16) * ((p.N + 63) / 64) >= 256;

@@ -165,7 +165,8 @@ SIZES = [(1, 1, 1), (1, 16, 128), (1, 300, 4100), (2, 17, 33), (3, 65, 129), (5,
          (64, 128, 384), (65, 129, 260), (127, 300, 200), (128, 256, 512), (130, 64, 1100), (140, 200, 128), (140, 200, 300), (140, 200, 900), (200, 520, 320), (256, 256, 128), (257, 511, 384), (300, 770, 129),
          (513, 1025, 640), (700, 512, 2048), (1, 9731, 200), (1100, 260, 130), (1093, 12113, 388), (4100, 3300, 640),
          (4, 200, 5000), (5, 300, 1000), (13, 17000, 136), (20, 200, 5000), (29, 9000, 264), (40, 300, 1032), (48, 12300, 136), (60, 4100, 264), (66, 9000, 900), (100, 12288, 264), (520, 3900, 520),
-         (1030, 4096, 264), (1100, 12288, 392)]
+         (1030, 4096, 264), (1100, 12288, 392),
+         (7, 100, 2), (9, 100, 5), (9, 100, 6), (9, 100, 10), (40, 130, 12), (40, 130, 262), (70, 130, 390), (70, 130, 396), (70, 130, 255), (600, 4096, 1001), (1030, 4096, 258), (1100, 12288, 271)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
