@@ -654,6 +654,8 @@ class Context:
         keep = [self._vector(post_weight, torch.bfloat16, dim, "post_weight"), self._vector(weight, torch.bfloat16, dim, "weight")]
         p.post_weight, p.weight = _ptr(keep[0]), _ptr(keep[1])
         for name, v in (("gate", gate), ("scale", scale), ("shift", shift)):
+            if v is None:
+                continue
             pair = tuple(v) if isinstance(v, (tuple, list)) else (v, v)
             if len(pair) != 2:
                 raise Flux2Error(L.ERR_INVALID_ARG, f"{name} must be one vector or a pair")

@@ -985,10 +985,35 @@ int pick_bf16_tile(const Mxfp4Gemm& p) {
     return best;
 }
 
-// 256 x 256 tiles, one per CU, or 128 x 128, two: measured, a group of 512 k of a round of 256 (512) tiles takes 4.4 (2.7) us, of up to 256 small ones 1.5.
-bool large_tiles(const Mxfp4Gemm& p) {
-    const int64_t big = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256), small = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128), rest = small % 512;
-    return (double)((big + 255) / 256) * 4.4 < (double)(small / 512) * 2.7 + (rest == 0 ? 0.0 : rest <= 256 ? 1.5 : 2.7);
+// MXFP4 x MXFP4 tiles.  Measured, us for a group of 512 k: a round of 256 large tiles (256 x 256, one per CU) 4.4, a round of 512 small ones (128 x 128,
+// two per CU) 2.7, of up to 256 of them 1.5; a second launch costs 3 us once.  Large tiles read half as much per product; where they leave most of their
+// last round empty, the columns of that round go to small ones (4608 x 4096 x 12288, 1.1 rounds: 146 -> 128 us; 4608 x 12288 x 4096, 3.4: 131 -> 129;
+// 4608 x 36864 x 4096, 10.1: 384 -> 389, hence the 6 %).
+double large_us(int64_t tiles) { return (double)((tiles + 255) / 256) * 4.4; }
+double small_us(int64_t tiles) {
+    const int64_t rest = tiles % 512;
+    return (double)(tiles / 512) * 2.7 + (rest == 0 ? 0.0 : rest <= 256 ? 1.5 : 2.7);
+}
+int launch_mxfp4_tiles(hipStream_t stream, const Mxfp4Gemm& p) {
+    const int64_t m2 = (p.M + 255) / 256, n2 = (p.N + 255) / 256, m1 = (p.M + 127) / 128, n1 = (p.N + 127) / 128;
+    const int64_t whole = m2 * n2 / 256 * 256 / m2;   // columns of large tiles in whole rounds
+    const double large = large_us(m2 * n2), small = small_us(m1 * n1);
+    const double both = whole > 0 && whole < n2 ? large_us(m2 * whole) + small_us(m1 * (n1 - 2 * whole)) + 3.0 * 4 / p.steps : 1e30;
+    if (both < 0.94 * large && both < small) {
+        Mxfp4Gemm a = p, b = p;
+        const int n = (int)whole * 256;
+        a.N = n;
+        b.N = p.N - n;
+        b.w += (int64_t)n * p.steps * 64;
+        b.w_scales += (int64_t)n * p.steps * 4;
+        if (p.bias) b.bias += n;
+        if (p.gate) b.gate += n;
+        if (p.resid) b.resid += n;
+        b.out = p.out_bf16 ? (void*)(reinterpret_cast<uint16_t*>(p.out) + n) : (void*)(reinterpret_cast<float*>(p.out) + n);
+        const int r = launch_tile<256, 256, 1>(stream, a);
+        return r ? r : launch_tile<128, 128, 2>(stream, b);
+    }
+    return large < small ? launch_tile<256, 256, 1>(stream, p) : launch_tile<128, 128, 2>(stream, p);
 }
 
 }  // namespace
@@ -1000,7 +1025,7 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
         // rows the tiles are faster as soon as there are 64 of them (32 x 12288 x 4096: 13.5 us against 18.1).
         if (p.M <= 16 || !offsets32) return launch_rows<1, 1, 4, 4>(stream, p);
         if (p.M <= 64 && p.N < 64 * 128) return launch_rows<2, 1, 4, 8>(stream, p);
-        return large_tiles(p) ? launch_tile<256, 256, 1>(stream, p) : launch_tile<128, 128, 2>(stream, p);
+        return launch_mxfp4_tiles(stream, p);
     }
     const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
     // few rows: A whole in LDS (1 x 19456 x 2560 8.5 us, 16-row tiles 11; at 16 rows 23.7 against 8.7)

@@ -6,8 +6,9 @@
 // gate, scale and shift are per column, one set for rows < split (text) and one for the others (image), as in layernorm_modulate.
 //
 // Bound by HBM: x and y are read once, x' and out written once; a row lives in the registers of the threads that own it, its statistics
-// are f32 sums over those registers (the variance around the mean of the row, in a second sum over registers, not E[x^2] - mean^2).  A thread owns at
-// most 16 values: wider rows get more threads, not more registers (12000 columns on 256 threads, 64 values each: 2.8 TB/s).
+// are f32 sums over those registers (the variance around the mean of the row, in a second sum over registers, not E[x^2] - mean^2).  What hides
+// the sums' and the vectors' latency is other rows' workgroups, so few registers count for more than early loads or vectors kept over several rows (both
+// measured: 5 to 40 % slower).
 // Rows may start at any element; f32 is moved 16 bytes at any dword, bf16 8 bytes at any dword and value by value where a row starts in the middle of one.
 #include "dev.h"
 #include "mxfp4.h"
@@ -174,17 +175,15 @@ int launch_form(hipStream_t stream, const ResidualNorm& p) {
 
 }  // namespace
 
-#ifndef D4
-#define D4 256, 4
-#define D8 512, 4
-#endif
 int launch_residual_norm(hipStream_t stream, const ResidualNorm& p) {
+    // 4608 x 4096: 53 us with 512 threads a row, 52 with 256, 65 with 1024; one row of 2560: 4.2, 5.3, 4.2.  4608 x 12000: 176 us with 512 threads of 32
+    // values, 212 with 1024 of 16, 235 with 256 of 64.
     if (p.dim <= 256) return launch_form<64, 1>(stream, p);
     if (p.dim <= 512) return launch_form<64, 2>(stream, p);
     if (p.dim <= 1024) return launch_form<256, 1>(stream, p);
     if (p.dim <= 2048) return launch_form<256, 2>(stream, p);
-    if (p.dim <= 4096) return launch_form<D4>(stream, p);
-    if (p.dim <= 8192) return launch_form<D8>(stream, p);
-    if (p.dim <= RESIDUAL_NORM_MAX_DIM) return launch_form<1024, 4>(stream, p);
+    if (p.dim <= 4096) return launch_form<512, 2>(stream, p);
+    if (p.dim <= 8192) return launch_form<512, 4>(stream, p);
+    if (p.dim <= RESIDUAL_NORM_MAX_DIM) return launch_form<512, 8>(stream, p);
     return 1;
 }

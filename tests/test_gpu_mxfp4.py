@@ -197,6 +197,18 @@ def test_epilogue(ctx, kind, m, n, k, bias, gate, resid):
         near(product(ctx, kind, a, w, **dev), want, bound, torch.bfloat16)
 
 
+@pytest.mark.parametrize("n,dtype", [(4100, torch.float32), (4104, torch.bfloat16)])
+def test_epilogue_over_both_tile_sizes(ctx, n, dtype):
+    """A product whose last columns go to the smaller tiles (18 x 17 large tiles are 1.2 rounds): every operand of the epilogue moves along."""
+    m, k = 4500, 260
+    a, w, a64, w64 = operands(ctx, "mxfp4", m, n, k)
+    g = gen(n)
+    b, s = torch.randn((n,), generator=g), torch.randn((n,), generator=g)
+    x = torch.randn((m, n), generator=g) if dtype == torch.float32 else None
+    want, bound = R.gemm(a64, w64, b, s, x)
+    near(ctx.op_gemm_mxfp4(a, w, bias=b.cuda(), gate=s.cuda(), resid=None if x is None else x.cuda(), dtype=dtype), want, bound, dtype)
+
+
 @pytest.mark.parametrize("kind", ["mxfp4", "bf16"])
 def test_product_is_not_transposed(ctx, kind):
     """The identity against a matrix of distinct code values: every element where it belongs, exactly."""
