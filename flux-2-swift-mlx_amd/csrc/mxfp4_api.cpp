@@ -27,13 +27,24 @@ struct DeviceScope {
 bool is_aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int elem_bytes(int dtype) { return dtype == FLUX2MI_F32 ? 4 : dtype == FLUX2MI_BF16 || dtype == FLUX2MI_F16 ? 2 : 0; }
 
-// address range of a [rows, cols] matrix of row stride ld (elements of esz bytes)
-struct Range { uintptr_t lo, hi; };
+// the memory of a [rows, cols] matrix of row stride ld (elements of esz bytes)
+struct Range { uintptr_t lo, hi, pitch, width; };
 Range range_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t esz) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    return p && rows > 0 && cols > 0 ? Range{lo, lo + (uintptr_t)(((rows - 1) * ld + cols) * esz)} : Range{lo, lo};
+    if (!p || rows <= 0 || cols <= 0) return Range{lo, lo, 0, 0};
+    uintptr_t last, hi;   // (no sizes wrap around: such a matrix reaches to the end of memory)
+    if (__builtin_mul_overflow((uintptr_t)(rows - 1), (uintptr_t)ld, &last) || __builtin_mul_overflow(last + (uintptr_t)cols, (uintptr_t)esz, &hi) ||
+        __builtin_add_overflow(lo, hi, &hi))
+        hi = UINTPTR_MAX;
+    return Range{lo, hi, (uintptr_t)ld * (uintptr_t)esz, (uintptr_t)cols * (uintptr_t)esz};
 }
-bool overlap(const Range& a, const Range& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Column slices of one buffer (equal pitch) reach into each other's range without sharing an element.
+bool overlap(const Range& a, const Range& b) {
+    if (a.lo >= b.hi || b.lo >= a.hi) return false;
+    if (a.pitch != b.pitch || a.width > a.pitch || b.width > a.pitch) return true;
+    const uintptr_t d = b.lo > a.lo ? (b.lo - a.lo) % a.pitch : (a.pitch - (a.lo - b.lo) % a.pitch) % a.pitch;   // b's first column in a's rows
+    return d < a.width || d + b.width > a.pitch;
+}
 Range codes_of(const void* p, int64_t rows, int64_t cols) { return range_of(p, 1, rows * (mxfp4_padded((int)cols) / 2), 0, 1); }
 Range scales_of(const void* p, int64_t rows, int64_t cols) { return range_of(p, 1, rows * (mxfp4_padded((int)cols) / 32), 0, 1); }
 

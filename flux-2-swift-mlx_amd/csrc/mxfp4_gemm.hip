@@ -677,7 +677,8 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
 // BM x BN outputs per workgroup of WM x WN waves.  A stage is one 128-k step: 256 bytes of every A row, 64 bytes of codes and 4 scale bytes of every
 // W row, all by LDS-DMA into a ring of STAGES buffers; STAGES - 1 of them are requested ahead and the wait is counted, so the stream is never drained.
 // W's codes become bf16 in registers (4 conversions per 8 values, used by MT MFMAs), a lane's scale is one byte of the row's four.
-// Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7, W: by (row / 2) & 3) so that fragment reads meet no bank conflicts.
+// Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7; W: the same where the codes of two steps come as one 128-byte line, else
+// the 64 bytes by (row / 2) & 3) so that fragment reads meet no bank conflicts.
 // A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead.  Columns >= K are zeroed where
 // the last stage is read or staged.
 __device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
@@ -893,8 +894,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void bf16_mxfp4_gemm_tile_kernel
     }
 }
 
-constexpr int64_t MAX_TILES = 1 << 22;   // x 512 threads: below 2^32 in a launch
-
 bool four_columns(const Mxfp4Gemm& p) {
     auto ok = [](const void* q, int64_t ld, int esz) { return !q || (reinterpret_cast<uintptr_t>(q) % (4 * esz) == 0 && ld % 4 == 0); };
     return p.N % 4 == 0 && ok(p.out, p.ld_out, p.out_bf16 ? 2 : 4) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
@@ -903,7 +902,6 @@ bool four_columns(const Mxfp4Gemm& p) {
 template <int MT, int NT, int U, int WAVES>
 int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
-    if (tn * tm >= MAX_TILES) return 1;
     const dim3 grid((unsigned)(tn * tm)), block(64 * WAVES);
     if (four_columns(p)) mxfp4_gemm_rows_kernel<true, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
     else mxfp4_gemm_rows_kernel<false, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
@@ -913,7 +911,6 @@ int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
 template <bool AVEC, int MT, int NT, int U, int WAVES>
 int launch_bf16_rows(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
-    if (tn * tm >= MAX_TILES) return 1;
     const int rows = p.M < 16 * MT ? p.M : 16 * MT, unit = WAVES * U;
     int chunk = 65536 / (rows * 256) / unit * unit;                    // A's part of LDS: 64 KB
     if (chunk < unit) chunk = unit;
@@ -930,7 +927,6 @@ int launch_bf16_rows(hipStream_t stream, const Mxfp4Gemm& p) {
 template <int BM, int BN, int PER_CU, bool BF16, bool VEC, int CUT>
 int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tn * tm >= MAX_TILES) return 1;
     constexpr int LDS = (BM + BN) * (2 * 128 + 3 * 16);
     const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, CUT, PER_CU>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
@@ -953,7 +949,6 @@ int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool AVEC, bool BF16, bool VEC>
 int launch_bf16_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tn * tm >= MAX_TILES) return 1;
     constexpr int NT = BN / (16 * WN), MT = BM / (16 * WM), TPG = 4 / KG, SBUF = (STAGES - 1 + TPG - 1) / TPG + 1;
     constexpr int RING = STAGES * KG * (BM * 256 + BN * 64) + SBUF * BN * 16, EPI = NT >= 4 ? WM * WN * 2 * store_slot_bytes<MT, NT, BF16>() : 0;
     constexpr int SUMS = (KG - 1) * WM * WN * NT * MT * 1024, LDS = RING > EPI ? (RING > SUMS ? RING : SUMS) : (EPI > SUMS ? EPI : SUMS);
@@ -985,6 +980,28 @@ int pick_bf16_tile(const Mxfp4Gemm& p) {
     return best;
 }
 
+// columns [0, n) and [n, N) of a product; rows [0, m) and [m, M)
+void cut_columns(const Mxfp4Gemm& p, int n, Mxfp4Gemm& a, Mxfp4Gemm& b) {
+    a = b = p;
+    a.N = n;
+    b.N = p.N - n;
+    b.w += (int64_t)n * p.steps * 64;
+    b.w_scales += (int64_t)n * p.steps * 4;
+    if (p.bias) b.bias += n;
+    if (p.gate) b.gate += n;
+    if (p.resid) b.resid += n;
+    b.out = reinterpret_cast<uint8_t*>(p.out) + (int64_t)n * (p.out_bf16 ? 2 : 4);
+}
+void cut_rows(const Mxfp4Gemm& p, int m, Mxfp4Gemm& a, Mxfp4Gemm& b) {
+    a = b = p;
+    a.M = m;
+    b.M = p.M - m;
+    b.a = reinterpret_cast<const uint8_t*>(p.a) + m * (p.a_scales ? (int64_t)p.steps * 64 : p.lda * 2);
+    if (p.a_scales) b.a_scales += (int64_t)m * p.steps * 4;
+    if (p.resid) b.resid += m * p.ld_resid;
+    b.out = reinterpret_cast<uint8_t*>(p.out) + m * p.ld_out * (p.out_bf16 ? 2 : 4);
+}
+
 // MXFP4 x MXFP4 tiles.  Measured, us for a group of 512 k: a round of 256 large tiles (256 x 256, one per CU) 4.4, a round of 512 small ones (128 x 128,
 // two per CU) 2.7, of up to 256 of them 1.5; a second launch costs 3 us once.  Large tiles read half as much per product; where they leave most of their
 // last round empty, the columns of that round go to small ones (4608 x 4096 x 12288, 1.1 rounds: 146 -> 128 us; 4608 x 12288 x 4096, 3.4: 131 -> 129;
@@ -1000,16 +1017,8 @@ int launch_mxfp4_tiles(hipStream_t stream, const Mxfp4Gemm& p) {
     const double large = large_us(m2 * n2), small = small_us(m1 * n1);
     const double both = whole > 0 && whole < n2 ? large_us(m2 * whole) + small_us(m1 * (n1 - 2 * whole)) + 3.0 * 4 / p.steps : 1e30;
     if (both < 0.94 * large && both < small) {
-        Mxfp4Gemm a = p, b = p;
-        const int n = (int)whole * 256;
-        a.N = n;
-        b.N = p.N - n;
-        b.w += (int64_t)n * p.steps * 64;
-        b.w_scales += (int64_t)n * p.steps * 4;
-        if (p.bias) b.bias += n;
-        if (p.gate) b.gate += n;
-        if (p.resid) b.resid += n;
-        b.out = p.out_bf16 ? (void*)(reinterpret_cast<uint16_t*>(p.out) + n) : (void*)(reinterpret_cast<float*>(p.out) + n);
+        Mxfp4Gemm a, b;
+        cut_columns(p, (int)whole * 256, a, b);
         const int r = launch_tile<256, 256, 1>(stream, a);
         return r ? r : launch_tile<128, 128, 2>(stream, b);
     }
@@ -1019,6 +1028,15 @@ int launch_mxfp4_tiles(hipStream_t stream, const Mxfp4Gemm& p) {
 }  // namespace
 
 int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
+    // A grid dimension holds 2^32 threads, a workgroup has at most 512 and covers at least 16 x 16 outputs: beyond 2^22 of those the longer side is halved
+    // (by then each half fills the chip many times over).
+    if (((int64_t)p.M + 15) / 16 * (((int64_t)p.N + 15) / 16) > 1 << 22) {
+        Mxfp4Gemm a, b;
+        if (p.N > p.M) cut_columns(p, p.N / 512 * 256, a, b);
+        else cut_rows(p, p.M / 512 * 256, a, b);
+        const int r = launch_mxfp4_gemm(stream, a);
+        return r ? r : launch_mxfp4_gemm(stream, b);
+    }
     const bool offsets32 = p.K < (1 << 24) && p.lda < (1 << 24);   // row offsets inside a tile fit 32 bits
     if (p.a_scales) {
         // up to 16 rows W is read once by 16-column workgroups: 4096 x 12288 8.8 us (one row); its 32 tiles of 128 columns would take 32.  Up to 64

@@ -117,8 +117,8 @@ template <int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(ResidualNorm p) {
     __shared__ float red[TPR / 64];
     const int t = threadIdx.x & (TPR - 1);
-    const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : (int64_t)blockIdx.x;
-    if (TPR == 64 && row >= p.rows) return;   // whole waves
+    const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, row = TPR == 64 ? group * 4 + threadIdx.x / 64 : group;
+    if (row >= p.rows) return;   // whole rows: TPR 64 has no barrier, the others' workgroups return as one
     const int dim = p.dim, set = row < p.split ? 0 : 1;
     float x[4 * NV], v[4 * NV];
     load_row<TPR, NV>(p.x + row * p.ldx, false, dim, t, x);
@@ -169,7 +169,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(Re
 template <int TPR, int NV>
 int launch_form(hipStream_t stream, const ResidualNorm& p) {
     constexpr int RPW = TPR == 64 ? 4 : 1;
-    residual_norm_kernel<TPR, NV><<<dim3((unsigned)((p.rows + RPW - 1) / RPW)), dim3(TPR * RPW), 0, stream>>>(p);
+    const unsigned groups = (unsigned)((p.rows + RPW - 1) / RPW), most = 1u << 22;   // x 512 threads: below the 2^32 of one grid dimension
+    residual_norm_kernel<TPR, NV><<<dim3(groups < most ? groups : most, (groups + most - 1) / most), dim3(TPR * RPW), 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 

@@ -279,6 +279,42 @@ def test_output_past_32_bits(ctx, kind):
 
 
 @pytest.mark.parametrize("kind", ["mxfp4", "bf16"])
+@pytest.mark.parametrize("m,n", [(1, (1 << 26) + 17), ((1 << 26) + 17, 1), (33000, 33100)])
+def test_more_outputs_than_a_launch_holds(ctx, flux2mi, kind, m, n):
+    """One column, so that an output is one product, exact in f32."""
+    g = torch.Generator("cuda").manual_seed(m)
+    a = torch.randint(-6, 7, (m, 1), generator=g, device="cuda").bfloat16()
+    w = ctx.op_quantize_mxfp4(torch.randint(1, 7, (n, 1), generator=g, device="cuda").float())
+    wv = ctx.op_dequantize_mxfp4(w, torch.float32)
+    if kind == "mxfp4":
+        a4 = ctx.op_quantize_mxfp4(a)
+        av = ctx.op_dequantize_mxfp4(a4, torch.float32)
+        out = ctx.op_gemm_mxfp4(a4, w, dtype=torch.float32)
+    else:
+        av = a.float()
+        out = ctx.op_gemm_bf16_mxfp4(a, w, dtype=torch.float32)
+    assert torch.equal(out, av * wv[:, 0])
+
+
+def test_column_slices_of_one_buffer(ctx):
+    """Operands and results beside each other in the rows of one buffer share no element."""
+    m, n, k = 37, 96, 160
+    a, w, a64, w64 = operands(ctx, "bf16", m, n, k)
+    f = torch.zeros((m, 300), device="cuda")
+    f[:, 5:5 + n] = 1.5
+    ctx.op_gemm_bf16_mxfp4(a, w, resid=f[:, 5:5 + n], out=f[:, 5 + n:5 + 2 * n])
+    want, bound = R.gemm(a64, w64, resid=torch.full((m, n), 1.5))
+    near(f[:, 5 + n:5 + 2 * n], want, bound, torch.float32)
+    assert (f[:, 5:5 + n] == 1.5).all() and not f[:, :5].any() and not f[:, 5 + 2 * n:].any()
+    h = torch.zeros((m, k + n), dtype=torch.bfloat16, device="cuda")
+    h[:, n:] = a
+    ctx.op_gemm_bf16_mxfp4(h[:, n:], w, out=h[:, :n])
+    want, bound = R.gemm(a64, w64)
+    near(h[:, :n], want, bound, torch.bfloat16)
+    assert torch.equal(h[:, n:], a)
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "bf16"])
 def test_same_result_every_time(ctx, kind):
     for m, n, k in ((1, 500, 3000), (40, 300, 3000), (300, 700, 1000)):
         a, w, _, _ = operands(ctx, kind, m, n, k)

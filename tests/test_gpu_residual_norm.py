@@ -135,3 +135,16 @@ def test_many_rows_past_32_bits(ctx):
     _, got = ctx.op_residual_norm(big, y.cuda(), post_norm="rms", weight=w.cuda())
     near(big, xs, xerr, torch.float32)
     near(got, out, oerr, torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,dim", [((1 << 24) - 1, 3), ((1 << 23) + 5, 2049)])
+def test_more_rows_than_a_grid_dimension_holds(ctx, rows, dim):
+    """Every row is updated once, in place."""
+    x = torch.full((rows, dim), 3.0, device="cuda")
+    gate = torch.arange(dim, device="cuda").float()
+    y = torch.ones((rows, dim), dtype=torch.bfloat16, device="cuda")
+    ctx.op_residual_norm(x, y, gate=gate, resid_scale=2.0, norm="none", want_out=False)
+    del y
+    want = 6.0 + gate
+    for at in range(0, rows, 1 << 20):
+        assert (x[at:at + (1 << 20)] == want).all(), at

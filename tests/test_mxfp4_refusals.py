@@ -80,6 +80,20 @@ def test_products(lib, ctx, kind, change, status, word):
         refuses(lib, lib.flux2mi_op_gemm_bf16_mxfp4(v["ctx"], v["a"], 70, *tail), status, word)
 
 
+def test_column_slices_that_share_a_column(lib, ctx):
+    """Rows of 100 f32: out is 40 columns from 30 on (or wraps into the next row's first ones), resid the first 40."""
+    call = lambda off: lib.flux2mi_op_gemm_bf16_mxfp4(ctx, A(0), 70, A(2), A(3), None, None, A(7) + 400, 100, A(7) + off, F32, 100, 9, 40, 70)  # noqa: E731
+    for column in (30, 39, 70 - 100, 99 - 100, 130, 170, 830):
+        refuses(lib, call(400 + 4 * column), INVALID, "overlap")
+
+
+@pytest.mark.parametrize("ld", [1 << 40, 1 << 61, (1 << 63) - 1])
+def test_row_strides_beyond_memory(flux2mi, lib, ctx, ld):
+    """Sizes whose bytes do not fit 64 bits, or reach over the other operands."""
+    refuses(lib, lib.flux2mi_op_quantize_mxfp4(ctx, A(0), F32, ld, 1 << 38, 64, A(1), A(2)), INVALID, "overlap")
+    refuses(lib, lib.flux2mi_op_gemm_bf16_mxfp4(ctx, A(0), ld, A(2), A(3), None, None, None, 0, A(7), F32, 40, 1 << 30, 40, 70), INVALID, "overlap")
+
+
 def test_products_first_operand(lib, ctx):
     tail = (A(2), A(3), None, None, None, 0, A(7), F32, 40, 9, 40, 70)
     refuses(lib, lib.flux2mi_op_gemm_mxfp4(ctx, None, A(1), *tail), INVALID, "A")
