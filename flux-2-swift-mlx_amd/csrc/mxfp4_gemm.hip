@@ -208,6 +208,11 @@ __device__ __forceinline__ void mfma_fp4_dma(u32x4 w, u32x4 a, f32x4& c, uint32_
 __device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
 }
+// not issued unless `wanted` (uniform): the branch is hidden in the asm, where it costs the compiler's schedule nothing
+__device__ __forceinline__ void dma16_if(bool wanted, uint32_t voff, const void* base, uint32_t lds) {
+    asm volatile("s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 skip%=\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\nskip%=:" ::"v"(voff), "s"(base), "s"(lds),
+                 "s"((int)wanted) : "memory", "scc");
+}
 __device__ __forceinline__ void dma4(uint32_t voff, const void* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
 }
@@ -216,9 +221,9 @@ __device__ __forceinline__ void lds_returned() { __builtin_amdgcn_s_waitcnt(0xc0
 // every piece but the FLYING youngest has landed, and every wave's LDS accesses are done
 template <int FLYING>
 __device__ __forceinline__ void hand_over() {
-    static_assert(FLYING < 16, "the low four bits of vmcnt");
+    static_assert(FLYING < 64, "vmcnt");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | FLYING);   // vmcnt FLYING, lgkmcnt 0
+    __builtin_amdgcn_s_waitcnt(0x0070 | (FLYING & 15) | (FLYING >> 4 << 14));   // vmcnt FLYING, lgkmcnt 0
     asm volatile("s_barrier" ::: "memory");
 }
 template <int MT, int NT>
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     constexpr int FREE = SLOTS / 2, EVERY = SLOTS * 3 / 2 / NP, FIRST = (SLOTS - FREE - 2) / EVERY + 1;   // FIRST: pieces requested in P0 (P2)
     static_assert(FREE + 1 + (NP - 1) * EVERY < 2 * SLOTS, "the last piece lies in the second phase");
     constexpr int SR = ROWS / 256;                         // scale rows per thread
-    extern __shared__ __align__(1024) uint8_t smem[];      // [2][STAGE] codes, [2][SCALES] scales, [SCALES] scales as they came
+    extern __shared__ __align__(1024) uint8_t smem[];      // [2][STAGE] codes, [2][SCALES] scales, [2 SCALES] two groups' scales as they came
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
     int tm, tn;
@@ -405,26 +410,35 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     auto back_of = [&](int stage) { return CUT != CUT_NONE && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
     auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + (k & ~3)) * 1024 : BN * 128 + (wave * PA + ((k - PW) & ~3)) * 1024); };
 
-    // Scales of a group: the 16 bytes [step][block] of row 64 wave + lane + 256 h come to LDS by DMA as they are; the same lane transposes them to
+    // Scales: the 16 bytes [step][block] of a row and group come to LDS by DMA as they are, two groups at a time (what counts is the lines touched, a
+    // third of them if every group's scales came alone: 4608 x 36864 x 4096 369 us, this way 356; 333 x 6144 x 18432 47.8, 44.2); the thread of the row transposes a group's to
     // one register per block with the steps as its bytes and writes [row / 64][block][row % 16][row / 16 % 4]: a fragment lane then reads the
     // registers of four row blocks at once.  (Loaded into registers instead, their use makes the compiler wait for every younger DMA piece too:
-    // 4608 x 36864 x 4096 388 us, this way 360.)
-    uint32_t vs[SR];
+    // 388 us against 360 when that was tried.)
+    uint32_t vs[2 * SR];
     const uint8_t* sbase[SR];
 #pragma unroll
-    for (int h = 0; h < SR; ++h) {
-        const int first = wave * 64 + 256 * h, row = (first < BN ? first : first - BN) + lane;
-        vs[h] = (uint32_t)(first < BN ? (row < last_w ? row : last_w) : (row < last_a ? row : last_a)) * row_scales;
+    for (int h = 0; h < SR; ++h) {   // piece 2 h + e: rows wave 64 + 256 h + 32 e ..., two lanes each; CUT_SHORT: piece 2 h, one lane per row
+        const int first = wave * 64 + 256 * h, row0 = first < BN ? first : first - BN, last = first < BN ? last_w : last_a;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = CUT == CUT_SHORT ? row0 + lane : row0 + 32 * e + (lane >> 1);
+            vs[2 * h + e] = (uint32_t)(row < last ? row : last) * row_scales;
+        }
         sbase[h] = first < BN ? p.w_scales + (int64_t)n0 * row_scales : p.a_scales + (int64_t)m0 * row_scales;
     }
     constexpr int RAW = 2 * STAGE + 2 * SCALES;
-    // a cut group's 16 bytes are the row's last ones, `skip` steps in front of the group's own; rows of fewer than four steps come dword by dword
-    auto skip_of = [&](int group) { return CUT == CUT_TAIL && group * 4 + 4 > steps ? group * 4 + 4 - steps : 0; };
-    auto fetch_scales = [&](int h, int group) {
+    // groups `group` and group + 1; a group that K cuts, or that lies behind it, comes as the row's last 16 bytes.  Rows of fewer than four steps: dword by dword
+    auto fetch_scales = [&](int i, int group, bool wanted) {
+        const int h = i >> 1;
         if constexpr (CUT == CUT_SHORT) {   // LDS: [step][row]
+            if (i & 1) return;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) dma4(vs[h], sbase[h] + (s < steps ? s : steps - 1) * 4, lds0 + RAW + h * 4096 + s * 1024 + wave * 256);
-        } else dma16(vs[h], sbase[h] + (group * 4 - skip_of(group)) * 4, lds0 + RAW + (h * 256 + wave * 64) * 16);   // LDS: [row][step]
+            for (int s = 0; s < 4; ++s) dma4(vs[i] + (s < steps ? s : steps - 1) * 4, sbase[h], lds0 + RAW + h * 4096 + s * 1024 + wave * 256);
+        } else {   // LDS: [row][group][step]
+            const uint32_t at = (uint32_t)group * 16 + (lane & 1) * 16, last = row_scales - 16;
+            dma16_if(wanted, vs[i] + (at < last ? at : last), sbase[h], lds0 + RAW + (h * 256 + wave * 64) * 32 + (i & 1) * 1024);
+        }
     };
     auto take_scales = [&](int h, int group) {   // steps behind K: 0
         u32x4 d;
@@ -435,9 +449,9 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
                 d[s] = s < steps ? v : 0u;
             }
         } else {
-            d = *reinterpret_cast<const u32x4*>(smem + RAW + (h * 256 + threadIdx.x) * 16);
-            if constexpr (CUT == CUT_TAIL) {
-                const int skip = skip_of(group);
+            d = *reinterpret_cast<const u32x4*>(smem + RAW + (h * 256 + threadIdx.x) * 32 + (group & 1) * 16);
+            if constexpr (CUT == CUT_TAIL) {   // a cut group's bytes lie `skip` steps further on
+                const int skip = group * 4 + 4 > steps ? group * 4 + 4 - steps : 0;
                 if (skip & 1) d = u32x4{d[1], d[2], d[3], 0u};
                 if (skip & 2) d = u32x4{d[2], d[3], 0u, 0u};
             }
@@ -485,6 +499,9 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     auto sw = [&](int j) { return sc[j / 4][j % 4]; };
     auto sa = [&](int i) { return sc[NT / 4 + i / 4][i % 4]; };
 
+    // one latency for the scales of two groups and two stages of codes; the second stage is still in flight when the loop begins
+#pragma unroll
+    for (int i = 0; i < 2 * SR; ++i) fetch_scales(i, 0, true);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         const int stage = b < last_stage ? b : last_stage;
@@ -492,17 +509,13 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
         for (int k = 0; k < NP; ++k)
             dma16((k < PW ? vw[k] : va[k - PW]) - back_of(stage), (k < PW ? wbase : abase) + stage * 128 + (k & 3) * 1024, code_lds(k, b) + (k & 3) * 1024);
     }
+    hand_over<NP>();
 #pragma unroll
-    for (int h = 0; h < SR; ++h) fetch_scales(h, 0);
-    hand_over<0>();
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int h = 0; h < SR; ++h) write_scales(h, take_scales(h, 0), 0);
+        for (int h = 0; h < SR; ++h) write_scales(h, take_scales(h, b), b);
     lds_returned();
-#pragma unroll
-    for (int h = 0; h < SR; ++h) fetch_scales(h, groups > 1 ? 1 : 0);
-    hand_over<0>();
-#pragma unroll
-    for (int h = 0; h < SR; ++h) write_scales(h, take_scales(h, groups > 1 ? 1 : 0), 1);
+    asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int t = 0; t < (NT + MT) / 4; ++t) sc[t] = read_scales(t, 0);
 #pragma unroll
@@ -513,11 +526,12 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
 
     // One loop body without a branch: behind the last group the requests repeat that group's.
     for (int q = 0; q < groups; ++q) {
-        const int qn = q + 1 < groups ? q + 1 : q, q2 = q + 2 < groups ? q + 2 : groups - 1;
+        const int qn = q + 1 < groups ? q + 1 : q;
         const int s0 = 2 * qn, s1 = 2 * qn + 1 < last_stage ? 2 * qn + 1 : last_stage;
         const uint8_t *w0 = wbase + s0 * 128, *a0 = abase + s0 * 128, *w1 = wbase + s1 * 128, *a1 = abase + s1 * 128;
         const uint32_t back0 = back_of(s0), back1 = back_of(s1);
-        // the scales of group q + 2 are requested in P1, have landed at the hand-over behind P2 and are transposed in P3, which reads those of group q + 1
+        // the scales of groups q + 2 and q + 3 (q even) are requested in P1 and have landed at the hand-over behind P2; P3 transposes those of group q + 2
+        // and reads those of group q + 1
         u32x4 raw[SR], next[(NT + MT) / 4];
         auto phase = [&](auto op) {
             constexpr int OP = decltype(op)::value, CUR = OP & 1, NBUF = OP == 1 || OP == 2 ? 1 : 0, NKS = OP & 1 ? 0 : 1;
@@ -532,13 +546,13 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
                     }
                 if constexpr (OP == 1) {   // in front of a piece that sets M0
 #pragma unroll
-                    for (int h = 0; h < SR; ++h)
-                        if (S == FREE + 1 + NP / 2 * EVERY - SLOTS - 1 - h) fetch_scales(h, q2);
+                    for (int i = 0; i < 2 * SR; ++i)
+                        if (S == FREE + 1 + NP / 2 * EVERY - SLOTS - 1 - i) fetch_scales(i, q + 2, !(q & 1));
                 }
                 if constexpr (OP == 3) {
 #pragma unroll
                     for (int h = 0; h < SR; ++h)
-                        if (S == SLOTS / 4 + h) raw[h] = take_scales(h, q2);
+                        if (S == SLOTS / 4 + h) raw[h] = take_scales(h, q + 2);
 #pragma unroll
                     for (int h = 0; h < SR; ++h)
                         if (S == SLOTS / 2 + 8 * h) write_scales(h, raw[h], q & 1);
@@ -927,7 +941,7 @@ int launch_bf16_rows(hipStream_t stream, const Mxfp4Gemm& p) {
 template <int BM, int BN, int PER_CU, bool BF16, bool VEC, int CUT>
 int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    constexpr int LDS = (BM + BN) * (2 * 128 + 3 * 16);
+    constexpr int LDS = (BM + BN) * (2 * 128 + 4 * 16);
     const auto fn = mxfp4_gemm_tile_kernel<BM, BN, BF16, VEC, CUT, PER_CU>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
     fn<<<dim3((unsigned)(tn * tm)), dim3(256), LDS, stream>>>(p, (int)tm, (int)tn, 6);
