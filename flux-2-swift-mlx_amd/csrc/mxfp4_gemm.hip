@@ -6,6 +6,8 @@
 // Operand layout (both forms): lane l of a wave holds row l % 16 of its 16-row block and the 32 values 32 (l / 16) ... of a 128-value step:
 // 16 bytes of codes = one MXFP4 block, so a lane needs one 16-byte load and one scale byte per step.  W is the MFMA's first operand: the
 // accumulator then holds 4 consecutive columns of one output row per lane (16-byte f32 / 8-byte bf16 stores).
+#include <algorithm>
+#include <cmath>
 #include <utility>
 
 #include "dev.h"
@@ -79,82 +81,44 @@ __device__ __forceinline__ bf16x8 load_a8(const uint16_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------------------------------------- few rows: K split over the waves of a workgroup
-// 16 MT rows x 16 NT columns per workgroup; its WAVES waves take the 128-value steps in turn (so that together they read whole lines of W) and
-// their sums are added in wave order through LDS.  Bound by reading W: operands go straight from memory to registers, U steps of a wave at a
-// time, and the next U are requested before the current ones are used.
-template <int MT, int NT>
-struct RowsStep {
-    u32x4 w[NT], a[MT];
-    uint32_t sw[NT], sa[MT];
-};
-
-template <bool VEC, int MT, int NT, int U, int WAVES>
+// 16 rows x 16 columns per workgroup; its WAVES waves take the 128-value steps in turn (so that together they read whole lines of W) and
+// their sums are added in wave order through LDS.  Bound by latency (8 x 2560 x 2560: 3.6 us) and, with more columns, by reading W: operands go straight
+// from memory to registers, U steps of a wave at a time, and the next U are requested before the current ones are used.
+template <bool VEC, int U, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n) {
-    __shared__ f32x4 part[WAVES][MT * NT][64];
+    __shared__ f32x4 part[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n0 = (int)(blockIdx.x % tiles_n) * 16 * NT, m0 = (int)(blockIdx.x / tiles_n) * 16 * MT;
-    const int64_t row_bytes = (int64_t)p.steps * 64, row_scales = (int64_t)p.steps * 4;
-    const int steps = p.steps;
-    const uint8_t *wq[NT], *ws[NT], *aq[MT], *as[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {   // rows behind the last one: its copy, never stored
-        const int64_t n = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
-        wq[j] = p.w + n * row_bytes + g * 16;
-        ws[j] = p.w_scales + n * row_scales + g;
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = m0 + 16 * i + r < p.M ? m0 + 16 * i + r : p.M - 1;
-        aq[i] = reinterpret_cast<const uint8_t*>(p.a) + m * row_bytes + g * 16;
-        as[i] = p.a_scales + m * row_scales + g;
-    }
-    auto load = [&](int s, RowsStep<MT, NT>& x) {
+    const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16, steps = p.steps;
+    const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1, m = m0 + r < p.M ? m0 + r : p.M - 1;   // rows behind the last one: its copy, never stored
+    const uint8_t *wq = p.w + n * steps * 64 + g * 16, *ws = p.w_scales + n * steps * 4 + g;
+    const uint8_t *aq = reinterpret_cast<const uint8_t*>(p.a) + m * steps * 64 + g * 16, *as = p.a_scales + m * steps * 4 + g;
+    struct Step { u32x4 w, a; uint32_t sw, sa; };
+    auto load = [&](int s, Step& x) {
         if (s >= steps) return;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            x.w[j] = *reinterpret_cast<const u32x4*>(wq[j] + (int64_t)s * 64);
-            x.sw[j] = ws[j][(int64_t)s * 4];
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            x.a[i] = *reinterpret_cast<const u32x4*>(aq[i] + (int64_t)s * 64);
-            x.sa[i] = as[i][(int64_t)s * 4];
-        }
+        x.w = *reinterpret_cast<const u32x4*>(wq + (int64_t)s * 64);
+        x.a = *reinterpret_cast<const u32x4*>(aq + (int64_t)s * 64);
+        x.sw = ws[(int64_t)s * 4];
+        x.sa = as[(int64_t)s * 4];
     };
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto use = [&](int s, const RowsStep<MT, NT>& x) {
-        if (s >= steps) return;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j][i] = mfma_fp4(x.w[j], x.a[i], acc[j][i], x.sw[j], x.sa[i]);
-    };
-    RowsStep<MT, NT> cur[U], next[U];
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    Step cur[U], next[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) load(wave + u * WAVES, cur[u]);
     for (int s = wave; s < steps; s += U * WAVES) {
 #pragma unroll
         for (int u = 0; u < U; ++u) load(s + (U + u) * WAVES, next[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) use(s + u * WAVES, cur[u]);
+        for (int u = 0; u < U; ++u)
+            if (s + u * WAVES < steps) acc = mfma_fp4(cur[u].w, cur[u].a, acc, cur[u].sw, cur[u].sa);
 #pragma unroll
         for (int u = 0; u < U; ++u) cur[u] = next[u];
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) part[wave][j * MT + i][lane] = acc[j][i];
+    part[wave][lane] = acc;
     __syncthreads();
-    for (int t = wave; t < MT * NT; t += WAVES) {
-        f32x4 v = part[0][t][lane];
+    if (wave) return;
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += part[w][t][lane];
-        store4<VEC>(p, m0 + 16 * (t % MT) + r, n0 + 16 * (t / MT) + 4 * g, v);
-    }
+    for (int w = 1; w < WAVES; ++w) acc += part[w][lane];
+    store4<VEC>(p, m0 + r, n0 + 4 * g, acc);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles staged through LDS (MXFP4 x MXFP4)
@@ -591,6 +555,120 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     else store_tile<MT, NT, BF16, VEC, false>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
 }
 
+// ---------------------------------------------------------------------------------------------- small tiles, k split over groups of waves
+// BM x BN outputs per workgroup of KG WM x WN waves: group kg of the waves takes the 128-k steps KG t + kg, and the groups' sums are added through LDS at
+// the end.  With few tiles a CU holds one, and a stage of it takes ~1200 cycles whatever its size (wait, barrier, LDS reads, MFMAs, requests: one wave per
+// SIMD issues them in turn), so what counts is how many k a stage holds: 32 x 64 tiles, 4096 k: two groups 11.4 us, four 7.4 (64 x 4096 outputs; the 128 x
+// 128 tiles above 11.9).  A stage is KG / 2 pairs of steps, a pair 128 bytes of every row (pieces and swizzle as above), in a ring of STAGES buffers,
+// STAGES - 1 of them requested ahead with a counted wait.  The scales of 16 steps come at once, one dword per row and step, ahead of the first of them;
+// slot c of a row holds step c ^ (row / 4) % 4 of the 16, so that the 16 rows a fragment reads lie in different banks.
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool BF16, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN * KG) void mxfp4_gemm_ring_kernel(Mxfp4Gemm p, int tiles_m, int tiles_n, int band) {
+    constexpr int WAVES = KG * WM * WN, MT = BM / (16 * WM), NT = BN / (16 * WN), ROWS = BM + BN;   // LDS rows of a stage: W's, then A's
+    constexpr int HALF = ROWS * 128, STAGE = KG / 2 * HALF, SCALES = ROWS * 64, CNT = KG * ROWS / 16 / WAVES, TPG = 16 / KG, NS = ROWS / 4 / WAVES;   // code pieces per wave and stage; scale pieces per wave and 16 steps
+    static_assert(CNT * 16 * WAVES == ROWS * KG && NS * 4 * WAVES == ROWS && BN % 8 == 0 && STAGES <= TPG / 2 + 2, "whole pieces; scales land in front of their use");
+    extern __shared__ __align__(1024) uint8_t smem[];   // [STAGES][STAGE] codes, [2][SCALES] scales
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % WM, wn = wave / WM % WN;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, band, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN, steps = p.steps, pairs = (steps + 1) >> 1, stages = (steps + KG - 1) / KG;
+    const uint32_t row_bytes = (uint32_t)steps * 64, row_scales = (uint32_t)steps * 4;
+    const uint8_t* wbase = p.w + (int64_t)n0 * row_bytes;
+    const uint8_t* abase = reinterpret_cast<const uint8_t*>(p.a) + (int64_t)m0 * row_bytes;
+    const uint8_t* wsbase = p.w_scales + (int64_t)n0 * row_scales;
+    const uint8_t* asbase = p.a_scales + (int64_t)m0 * row_scales;
+    const int last_w = p.N - 1 - n0, last_a = p.M - 1 - m0;   // rows behind the last one: its copy, never stored
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    auto clamped = [&](int row) { return (uint32_t)(row < BN ? (row < last_w ? row : last_w) : (row - BN < last_a ? row - BN : last_a)); };
+
+    const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    uint32_t vc[CNT];
+#pragma unroll
+    for (int k = 0; k < CNT; ++k) vc[k] = clamped((wave * CNT + k) % (ROWS / 8) * 8 + (lane >> 3)) * row_bytes + chunk;
+    auto issue = [&](int t, int buf) {   // stage t; behind the end the last one again, so that every stage counts alike
+        // the second step of the last pair may lie behind the row: its chunks are then fetched from the first step, and not used
+        const uint32_t cut = (steps & 1) && chunk >= 64 ? 64u : 0u;
+#pragma unroll
+        for (int k = 0; k < CNT; ++k) {
+            const int piece = wave * CNT + k, want = t * (KG / 2) + piece / (ROWS / 8), pair = want < pairs ? want : pairs - 1;
+            dma16(vc[k] - (pair == pairs - 1 ? cut : 0u), (piece % (ROWS / 8) * 8 < BN ? wbase : abase) + (int64_t)pair * 128, lds0 + buf * STAGE + piece * 1024);
+        }
+    };
+    auto issue_scales = [&](int group, int j) {
+        const int piece = wave * NS + j, row = piece * 4 + (lane >> 4), s = group * 16 + ((lane & 15) ^ (piece & 3)), step = s < steps ? s : steps - 1;
+        dma4(clamped(row) * row_scales + (uint32_t)step * 4, piece * 4 < BN ? wsbase : asbase, lds0 + STAGES * STAGE + (group & 1) * SCALES + piece * 256);
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int s, int buf) {
+        const uint8_t* c = smem + buf * STAGE + kg / 2 * HALF + (((kg & 1) * 4 + g) ^ (r & 7)) * 16;
+        const uint8_t* sc = smem + STAGES * STAGE + (s >> 4 & 1) * SCALES + ((s & 15) ^ (r >> 2)) * 4 + g;
+        const int wrow = wn * NT * 16 + r, arow = BN + wm * MT * 16 + r;
+        u32x4 w[NT], a[MT];
+        uint32_t sw[NT], sa[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            w[j] = *reinterpret_cast<const u32x4*>(c + (wrow + 16 * j) * 128);
+            sw[j] = sc[(wrow + 16 * j) * 64];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            a[i] = *reinterpret_cast<const u32x4*>(c + (arow + 16 * i) * 128);
+            sa[i] = sc[(arow + 16 * i) * 64];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j][i] = mfma_fp4(w[j], a[i], acc[j][i], sw[j], sa[i]);
+    };
+#pragma unroll
+    for (int j = 0; j < NS; ++j) issue_scales(0, j);
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) issue(t, t);
+    int buf = 0, before = STAGES - 1;   // t % STAGES, (t - 1) % STAGES
+    for (int t = 0; t < stages; ++t) {
+        hand_over<(STAGES - 2) * CNT>();   // stage t has landed (scale pieces in flight come on top: it then waits for that much more, never for less)
+        const int turn = t % TPG;
+        if (turn < TPG / 2) {              // the next 16 steps' scales, into the buffer that the previous 16 have left
+            constexpr int EACH = (NS + TPG / 2 - 1) / (TPG / 2);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j)
+                if (turn * EACH + j < NS) issue_scales(t / TPG + 1, turn * EACH + j);
+        }
+        issue(t + STAGES - 1, before);     // into the buffer of stage t - 1, which everybody has left
+        if (KG * t + kg < steps) compute(KG * t + kg, buf);
+        before = buf;
+        buf = buf + 1 < STAGES ? buf + 1 : 0;
+    }
+    hand_over<0>();
+    f32x4* part = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+    for (int half = KG / 2; half >= 1; half /= 2) {   // the k groups' sums, the upper half's added to the lower's
+        if (kg >= half && kg < 2 * half) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) part[((wave - half * WM * WN) * NT * MT + j * MT + i) * 64 + lane] = acc[j][i];
+        }
+        __syncthreads();
+        if (kg < half) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] += part[(wave * NT * MT + j * MT + i) * 64 + lane];
+        }
+        __syncthreads();
+    }
+    if (kg > 0) return;
+    uint8_t* mine = smem + wave * 2 * store_slot_bytes<MT, NT, BF16>();
+    if (p.bias || p.gate) store_tile<MT, NT, BF16, VEC, true>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    else store_tile<MT, NT, BF16, VEC, false>(p, acc, mine, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+}
+
 // rows of out and resid take 16-byte accesses of the columns a lane of store_tile owns (8 of bf16, 4 of f32)
 bool wide_rows(const Mxfp4Gemm& p) {
     auto ok = [](const void* q, int64_t ld, int cols) { return !q || (reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % cols == 0); };
@@ -913,12 +991,12 @@ bool four_columns(const Mxfp4Gemm& p) {
     return p.N % 4 == 0 && ok(p.out, p.ld_out, p.out_bf16 ? 2 : 4) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
 }
 
-template <int MT, int NT, int U, int WAVES>
 int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
-    const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
-    const dim3 grid((unsigned)(tn * tm)), block(64 * WAVES);
-    if (four_columns(p)) mxfp4_gemm_rows_kernel<true, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
-    else mxfp4_gemm_rows_kernel<false, MT, NT, U, WAVES><<<grid, block, 0, stream>>>(p, (int)tn);
+    constexpr int U = 4, WAVES = 4;
+    const int tn = (p.N + 15) / 16, tm = (p.M + 15) / 16;
+    const dim3 grid((unsigned)(tn * (int64_t)tm)), block(64 * WAVES);
+    if (four_columns(p)) mxfp4_gemm_rows_kernel<true, U, WAVES><<<grid, block, 0, stream>>>(p, tn);
+    else mxfp4_gemm_rows_kernel<false, U, WAVES><<<grid, block, 0, stream>>>(p, tn);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
@@ -958,6 +1036,24 @@ int launch_tile(hipStream_t stream, const Mxfp4Gemm& p) {
     const bool vec = wide_rows(p);
     if (p.out_bf16) return vec ? launch_tile_cut<BM, BN, PER_CU, true, true>(stream, p) : launch_tile_cut<BM, BN, PER_CU, true, false>(stream, p);
     return vec ? launch_tile_cut<BM, BN, PER_CU, false, true>(stream, p) : launch_tile_cut<BM, BN, PER_CU, false, false>(stream, p);
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool BF16, bool VEC>
+int launch_ring_form(hipStream_t stream, const Mxfp4Gemm& p) {
+    const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+    constexpr int NT = BN / (16 * WN), MT = BM / (16 * WM), RING = (BM + BN) * (STAGES * KG * 64 + 2 * 64);
+    constexpr int EPI = WM * WN * 2 * store_slot_bytes<MT, NT, BF16>(), SUMS = KG / 2 * WM * WN * NT * MT * 1024, LDS = RING > EPI ? (RING > SUMS ? RING : SUMS) : (EPI > SUMS ? EPI : SUMS);
+    static_assert(LDS <= 163840, "160 KB");
+    const auto fn = mxfp4_gemm_ring_kernel<BM, BN, WM, WN, KG, STAGES, BF16, VEC>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 2;
+    fn<<<dim3((unsigned)(tn * tm)), dim3(64 * WM * WN * KG), LDS, stream>>>(p, (int)tm, (int)tn, 6);
+    return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+template <int BM, int BN, int WM, int WN, int KG, int STAGES>
+int launch_ring(hipStream_t stream, const Mxfp4Gemm& p) {
+    const bool vec = wide_rows(p);
+    if (p.out_bf16) return vec ? launch_ring_form<BM, BN, WM, WN, KG, STAGES, true, true>(stream, p) : launch_ring_form<BM, BN, WM, WN, KG, STAGES, true, false>(stream, p);
+    return vec ? launch_ring_form<BM, BN, WM, WN, KG, STAGES, false, true>(stream, p) : launch_ring_form<BM, BN, WM, WN, KG, STAGES, false, false>(stream, p);
 }
 
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool AVEC, bool BF16, bool VEC>
@@ -1039,6 +1135,19 @@ int launch_mxfp4_tiles(hipStream_t stream, const Mxfp4Gemm& p) {
     return large < small ? launch_tile<256, 256, 1>(stream, p) : launch_tile<128, 128, 2>(stream, p);
 }
 
+// Small tiles or those above: a fixed part and one per 512 k, us, for as many tiles as there are CUs, fitted to 1 ... 512 rows x 2560 ... 36864 outputs x
+// 1024 ... 16384 k.  16 x 64 tiles have two workgroups per CU.  What the choice gives, us: 64 x 4096 x 4096 6.5 / 7.6 / 8.6 (16 x 64 / 32 x 64 / 32 x 128)
+// and 11.9 (128 x 128), 128 x 4096 x 4096 8.6 / 7.8 / 8.9 and 12.4, 256 x 4096 x 4096 15.3 / 14.3 / 9.4 and 13.1, 384 x 4096 x 4096 21.7 / 20.4 / 16.7 and 13.4.
+enum Ring { RING_NONE, RING_16, RING_32, RING_32_WIDE };
+Ring pick_ring(const Mxfp4Gemm& p) {
+    auto tiles = [&](int bm, int bn) { return (double)(((p.M + bm - 1) / bm) * (int64_t)((p.N + bn - 1) / bn)); };
+    const double groups = p.steps / 4.0, n16 = tiles(16, 64), n128 = tiles(128, 128);
+    if (n128 > 512) return RING_NONE;
+    const double us[] = {3.0 + (n128 <= 256 ? 1.1 : 2.2) * groups, (2.9 + 0.41 * groups) * (n16 <= 256 ? 1.0 : n16 <= 512 ? 1.35 : 0.55 + 0.42 * n16 / 256),
+                         (3.9 + 0.44 * groups) * std::ceil(tiles(32, 64) / 256), (4.1 + 0.56 * groups) * std::ceil(tiles(32, 128) / 256)};
+    return (Ring)(std::min_element(us, us + 4) - us);
+}
+
 }  // namespace
 
 int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
@@ -1053,10 +1162,15 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
     }
     const bool offsets32 = p.K < (1 << 24) && p.lda < (1 << 24);   // row offsets inside a tile fit 32 bits
     if (p.a_scales) {
-        // up to 16 rows W is read once by 16-column workgroups: 4096 x 12288 8.8 us (one row); its 32 tiles of 128 columns would take 32.  Up to 64
-        // rows the tiles are faster as soon as there are 64 of them (32 x 12288 x 4096: 13.5 us against 18.1).
-        if (p.M <= 16 || !offsets32) return launch_rows<1, 1, 4, 4>(stream, p);
-        if (p.M <= 64 && p.N < 64 * 128) return launch_rows<2, 1, 4, 8>(stream, p);
+        // Up to 16 rows of at most 4096 outputs (a 16-column workgroup per CU): 8 x 2560 x 2560 3.6 us, 16 x 64 tiles 5.2; 8 x 12288 x 4096 11.0, 7.0.
+        // Up to 4 rows also of more outputs while k is short: 1 x 19456 x 2560 7.3 us, 8.2; 1 x 12288 x 4096 8.6, 6.9.
+        if ((p.M <= 16 && p.N <= 4096) || (p.M <= 4 && p.steps <= 24) || !offsets32) return launch_rows(stream, p);
+        switch (pick_ring(p)) {
+            case RING_16: return launch_ring<16, 64, 1, 1, 4, 3>(stream, p);
+            case RING_32: return launch_ring<32, 64, 1, 1, 4, 3>(stream, p);
+            case RING_32_WIDE: return launch_ring<32, 128, 1, 2, 4, 3>(stream, p);
+            case RING_NONE: break;
+        }
         return launch_mxfp4_tiles(stream, p);
     }
     const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
