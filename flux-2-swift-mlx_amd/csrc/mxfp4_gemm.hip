@@ -138,6 +138,9 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p
 // With one wave per SIMD every instruction takes an issue slot of ~5 cycles and an MFMA 16, so the side work goes between single MFMAs ("slots"),
 // about one instruction at a time (measured: what an instruction costs beyond that is 4 cycles each).
 // A lane's four scale bytes of a group (one per step) are one register, the byte is chosen by the MFMA's op_sel.
+// Measured: 4608 x 36864 x 4096 354 us = 3.9 PF, 4608 x 16384 x 16384 529 us = 4.7 PF.  Bound by the matrix pipe's power and by the delivery L2 -> LDS
+// together: a group takes 3.5 us, without its requests 2.5, without its LDS reads 3.4, without either 2.4 (7.3 PF, the clock down to 1.8 GHz; the same
+// loop on zero operands: 2.8, 1.9 without requests).  A tile's prologue and its output take 8 us.
 // Steps behind K: addresses stay inside the row and both scale bytes are 0, 2^-254 times finite codes, which is below f32: exactly 0.
 //
 // The MFMA is asm with the accumulator pinned to AGPRs: left to itself the register allocator of a one-wave-per-SIMD kernel moves accumulators
@@ -558,8 +561,8 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
 // ---------------------------------------------------------------------------------------------- small tiles, k split over groups of waves
 // BM x BN outputs per workgroup of KG WM x WN waves: group kg of the waves takes the 128-k steps KG t + kg, and the groups' sums are added through LDS at
 // the end.  With few tiles a CU holds one, and a stage of it takes ~1200 cycles whatever its size (wait, barrier, LDS reads, MFMAs, requests: one wave per
-// SIMD issues them in turn), so what counts is how many k a stage holds: 32 x 64 tiles, 4096 k: two groups 11.4 us, four 7.4 (64 x 4096 outputs; the 128 x
-// 128 tiles above 11.9).  A stage is KG / 2 pairs of steps, a pair 128 bytes of every row (pieces and swizzle as above), in a ring of STAGES buffers,
+// SIMD issues them in turn), so what counts is how many k a stage holds: 64 x 4096 x 4096 with 64 x 64 tiles and two groups 11.3 us, four 9.4, four and 32 x 64
+// tiles 7.4 (the 128 x 128 tiles above 11.9).  Bound by that latency: 16 x 36864 x 4096 17.6 us = 4.6 TB/s of W, 16 x 12288 x 4096 7.2.  A stage is KG / 2 pairs of steps, a pair 128 bytes of every row (pieces and swizzle as above), in a ring of STAGES buffers,
 // STAGES - 1 of them requested ahead with a counted wait.  The scales of 16 steps come at once, one dword per row and step, ahead of the first of them;
 // slot c of a row holds step c ^ (row / 4) % 4 of the 16, so that the 16 rows a fragment reads lie in different banks.
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool BF16, bool VEC>
@@ -679,6 +682,7 @@ bool wide_rows(const Mxfp4Gemm& p) {
 // A is shared by every wave of a workgroup and comes once per workgroup through LDS, `chunk` steps of all its rows at a time (chunk % WAVES == 0, so
 // that a wave's steps wave, wave + WAVES, ... fall into the chunks alike); W and its scales stream through registers across the chunks.
 // Read by every wave for itself, A costs four loads per step against one of W: the vector-memory path, not HBM, is then the bound.
+// Measured: 1 x 19456 x 2560 8.6 us = 3.1 TB/s of W; bound by the latency of staging A and of a wave's first loads.
 template <bool AVEC, bool VEC, int MT, int NT, int U, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n, int chunk) {
     extern __shared__ __align__(16) uint8_t smem[];   // A: [rows][chunk * 256 + 16] bytes; then the partial sums [WAVES][MT * NT][64]
@@ -771,7 +775,9 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
 // W's codes become bf16 in registers (4 conversions per 8 values, used by MT MFMAs), a lane's scale is one byte of the row's four.
 // Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7; W: the same where the codes of two steps come as one 128-byte line, else
 // the 64 bytes by (row / 2) & 3) so that fragment reads meet no bank conflicts.
-// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead.  Columns >= K are zeroed where
+// Measured: 23 x 5120 x 5120 9.1 us, 512 x 4096 x 12288 53 us = 0.97 PF, 4608 x 12288 x 4096 370 us = 1.25 PF; bound by the conversions, which share the
+// issue slots with the MFMAs, and with few rows by the latency of a stage.
+// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead (512 x 4096 x 12283: 132 us).  Columns >= K are zeroed where
 // the last stage is read or staged.
 __device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
     u32x4 u = __builtin_bit_cast(u32x4, v);
