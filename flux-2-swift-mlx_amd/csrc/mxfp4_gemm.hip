@@ -363,16 +363,17 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
     const int steps = p.steps, groups = (steps + 3) >> 2, last_stage = (steps - 1) >> 1;
 
     // DMA sources relative to the stage's column: lane l fetches chunk (l % 8) ^ (row % 8) of row l / 8 of its piece.  Four pieces share one M0: the
-    // instruction's offset goes to both addresses, so piece k of them starts 1024 k further in LDS and its source offset carries -1024 k (+ 3072 so
-    // that it stays unsigned; the scalar base is 3072 lower).
+    // instruction's offset goes to both addresses, so piece k of them starts 1024 k further in LDS and its source offset carries -1024 k (+ LOWER so
+    // that it stays unsigned; the scalar base is LOWER lower).
+    constexpr uint32_t LOWER = 3 * 1024;
     uint32_t vw[PW], va[PA];
     const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
-    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes + chunk + 3072 - (k & 3) * 1024; }
+    for (int k = 0; k < PW; ++k) { const int row = (wave * PW + k) * 8 + (lane >> 3); vw[k] = (uint32_t)(row < last_w ? row : last_w) * row_bytes + chunk + LOWER - (k & 3) * 1024; }
 #pragma unroll
-    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes + chunk + 3072 - (k & 3) * 1024; }
-    wbase -= 3072;
-    abase -= 3072;
+    for (int k = 0; k < PA; ++k) { const int row = (wave * PA + k) * 8 + (lane >> 3); va[k] = (uint32_t)(row < last_a ? row : last_a) * row_bytes + chunk + LOWER - (k & 3) * 1024; }
+    wbase -= LOWER;
+    abase -= LOWER;
     // the second step of the last stage may lie behind the row: its chunks are then fetched from the first step (their scales are 0)
     auto back_of = [&](int stage) { return CUT != CUT_NONE && stage == last_stage && (steps & 1) && chunk >= 64 ? 64u : 0u; };
     auto code_lds = [&](int k, int buf) { return lds0 + buf * STAGE + (k < PW ? (wave * PW + (k & ~3)) * 1024 : BN * 128 + (wave * PA + ((k - PW) & ~3)) * 1024); };
