@@ -1082,19 +1082,19 @@ int launch_bf16_tile(hipStream_t stream, const Mxfp4Gemm& p) {
     return vec ? launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, false, true>(stream, p) : launch_bf16_tile_form<BM, BN, WM, WN, KG, STAGES, AVEC, false, false>(stream, p);
 }
 
-// Tile of A in bf16: the launch's rounds (256 CUs, a workgroup each) x what a 128-k step of a full round takes, us, measured at 64 ... 4608 rows x 4096 /
-// 12288 columns.  A larger tile does more per step and byte, a smaller one fills the chip at fewer rows.
-struct Bf16Tile { int bm, bn; double us; };
-constexpr Bf16Tile BF16_TILES[] = {{32, 128, 0.35}, {64, 128, 0.56}, {64, 256, 0.97}, {128, 256, 1.70}};
-int pick_bf16_tile(const Mxfp4Gemm& p) {
-    int best = 0;
-    double least = 1e30;
-    for (int i = 0; i < 4; ++i) {
-        const int64_t tiles = (int64_t)((p.M + BF16_TILES[i].bm - 1) / BF16_TILES[i].bm) * ((p.N + BF16_TILES[i].bn - 1) / BF16_TILES[i].bn);
-        const double t = (double)((tiles + 255) / 256) * BF16_TILES[i].us;
-        if (t < least) { least = t; best = i; }
-    }
-    return best;
+// Tile of A in bf16: rounds of 256 tiles (a CU each; 16-row tiles have two workgroups per CU) x a fixed part and one per 128-k step, us, fitted to 16 ... 512
+// rows x 2560 ... 19456 outputs x 2560 ... 9728 k and to 4608 rows.  With few tiles more k groups count (what a stage takes is latency), with many the
+// products per byte.  What the choice gives, us: 64 x 4096 x 4096 8.6 (16 x 32), 9.7 (32 x 64), 12.2 (32 x 128); 128 x 4096 x 4096 15.3, 10.2, 12.6;
+// 256 x 4096 x 4096 26.2, 18.9, 13.6; 128 x 12288 x 4096 38, 27, 24 and 20.0 (64 x 128).
+enum Bf16Tile { BF16_16x32, BF16_16x64, BF16_32x64, BF16_32x128, BF16_64x128, BF16_64x256, BF16_128x256 };
+Bf16Tile pick_bf16_tile(const Mxfp4Gemm& p) {
+    auto tiles = [&](int bm, int bn) { return (double)(((p.M + bm - 1) / bm) * (int64_t)((p.N + bn - 1) / bn)); };
+    auto two = [](double n) { return n <= 256 ? 1.0 : n <= 512 ? 1.36 : 0.7 + 0.51 * n / 256; };
+    const double s = p.steps;
+    const double us[] = {(3.35 + 0.08 * s) * two(tiles(16, 32)), (3.2 + 0.163 * s) * two(tiles(16, 64)), (4.05 + 0.172 * s) * std::ceil(tiles(32, 64) / 256),
+                         (4.3 + 0.24 * s) * std::ceil(tiles(32, 128) / 256), (4.0 + 0.5 * s) * std::ceil(tiles(64, 128) / 256),
+                         (4.0 + 0.86 * s) * std::ceil(tiles(64, 256) / 256), (4.0 + 1.72 * s) * std::ceil(tiles(128, 256) / 256)};
+    return (Bf16Tile)(std::min_element(us, us + 7) - us);
 }
 
 // columns [0, n) and [n, N) of a product; rows [0, m) and [m, M)
@@ -1184,16 +1184,20 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
     // few rows: A whole in LDS (1 x 19456 x 2560 8.5 us, 16-row tiles 11; at 16 rows 23.7 against 8.7)
     if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true, 1, 1, 2, 8>(stream, p) : launch_bf16_rows<false, 1, 1, 2, 8>(stream, p);
     const bool dma = reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && p.lda % 2 == 0 && p.K % 2 == 0 && p.K >= 8;   // A by DMA, or through registers
-    if (p.M <= 32) {
-        // 16-row tiles; 64 columns as soon as these fill the chip, else 32 and four k groups (23 x 5120 x 5120: 9.0 us against 9.9; 16 x 19456 x 2560: 9.8, 8.7)
-        const bool wide = (int64_t)((p.M + 15) / 16) * ((p.N + 63) / 64) >= 256;
-        if (wide) return dma ? launch_bf16_tile<16, 64, 1, 4, 2, 3, true>(stream, p) : launch_bf16_tile<16, 64, 1, 4, 2, 3, false>(stream, p);
-        return dma ? launch_bf16_tile<16, 32, 1, 2, 4, 3, true>(stream, p) : launch_bf16_tile<16, 32, 1, 2, 4, 3, false>(stream, p);
+    const Bf16Tile tile = pick_bf16_tile(p);
+    if (!dma) {   // (A's way through registers bounds these: fewer forms)
+        if (tile == BF16_128x256) return launch_bf16_tile<128, 256, 2, 4, 1, 3, false>(stream, p);
+        if (p.M > 32) return launch_bf16_tile<64, 128, 1, 4, 2, 3, false>(stream, p);
+        return tile == BF16_16x32 ? launch_bf16_tile<16, 32, 1, 2, 4, 3, false>(stream, p) : launch_bf16_tile<16, 64, 1, 4, 2, 3, false>(stream, p);
     }
-    const int tile = pick_bf16_tile(p);
-    if (!dma) return tile == 3 ? launch_bf16_tile<128, 256, 2, 4, 1, 3, false>(stream, p) : launch_bf16_tile<64, 128, 1, 4, 2, 3, false>(stream, p);
-    if (tile == 0) return launch_bf16_tile<32, 128, 1, 4, 2, 3, true>(stream, p);
-    if (tile == 1) return launch_bf16_tile<64, 128, 1, 4, 2, 3, true>(stream, p);
-    if (tile == 2) return launch_bf16_tile<64, 256, 1, 4, 2, 2, true>(stream, p);
+    switch (tile) {
+        case BF16_16x32: return launch_bf16_tile<16, 32, 1, 2, 4, 3, true>(stream, p);
+        case BF16_16x64: return launch_bf16_tile<16, 64, 1, 4, 2, 3, true>(stream, p);
+        case BF16_32x64: return launch_bf16_tile<32, 64, 1, 2, 4, 3, true>(stream, p);
+        case BF16_32x128: return launch_bf16_tile<32, 128, 1, 4, 4, 2, true>(stream, p);
+        case BF16_64x128: return launch_bf16_tile<64, 128, 1, 4, 2, 3, true>(stream, p);
+        case BF16_64x256: return launch_bf16_tile<64, 256, 1, 4, 2, 2, true>(stream, p);
+        case BF16_128x256: break;
+    }
     return launch_bf16_tile<128, 256, 2, 4, 1, 3, true>(stream, p);
 }

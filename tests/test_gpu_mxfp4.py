@@ -198,18 +198,19 @@ def test_epilogue(ctx, kind, m, n, k, bias, gate, resid):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 4112, 128), (13, 4200, 129), (16, 5003, 2600), (30, 1000, 300), (40, 200, 4200), (100, 5120, 1100), (128, 4096, 700), (33, 12290, 520),
-                                   (190, 4100, 2050), (250, 3000, 4480), (64, 64, 16000)])
+                                   (190, 4100, 2050), (250, 3000, 4480), (64, 64, 16000), (20, 12290, 4098), (90, 4090, 2562), (200, 5000, 1030), (129, 4096, 1412)])
 @pytest.mark.parametrize("every", [False, True])
-def test_product_of_few_rows(ctx, m, n, k, every):
+@pytest.mark.parametrize("kind", ["mxfp4", "bf16"])
+def test_product_of_few_rows(ctx, kind, m, n, k, every):
     """Sizes where k is split over groups of waves: steps that do not fill a stage, ragged tiles, each epilogue."""
-    a, w, a64, w64 = operands(ctx, "mxfp4", m, n, k)
+    a, w, a64, w64 = operands(ctx, kind, m, n, k)
     g = gen(m, n, k, 9)
     bias, gate, resid = (torch.randn(n, generator=g), torch.randn(n, generator=g), torch.randn((m, n), generator=g)) if every else (None, None, None)
     cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
     want, bound = R.gemm(a64, w64, bias, gate, resid)
-    near(product(ctx, "mxfp4", a, w, bias=cuda(bias), gate=cuda(gate), resid=cuda(resid), dtype=torch.float32), want, bound, torch.float32)
+    near(product(ctx, kind, a, w, bias=cuda(bias), gate=cuda(gate), resid=cuda(resid), dtype=torch.float32), want, bound, torch.float32)
     want, bound = R.gemm(a64, w64, bias, gate)
-    near(product(ctx, "mxfp4", a, w, bias=cuda(bias), gate=cuda(gate)), want, bound, torch.bfloat16)
+    near(product(ctx, kind, a, w, bias=cuda(bias), gate=cuda(gate)), want, bound, torch.bfloat16)
 
 
 @pytest.mark.parametrize("n,dtype", [(4100, torch.float32), (4104, torch.bfloat16)])
