@@ -778,7 +778,7 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
 // the 64 bytes by (row / 2) & 3) so that fragment reads meet no bank conflicts.
 // Measured: 23 x 5120 x 5120 9.1 us, 512 x 4096 x 12288 53 us = 0.97 PF, 4608 x 12288 x 4096 370 us = 1.25 PF; bound by the conversions, which share the
 // issue slots with the MFMAs, and with few rows by the latency of a stage.
-// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead (512 x 4096 x 12283: 132 us).  Columns >= K are zeroed where
+// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead (512 x 4096 x 4095: 40 us, x 4096 21).  Columns >= K are zeroed where
 // the last stage is read or staged.
 __device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
     u32x4 u = __builtin_bit_cast(u32x4, v);
@@ -1185,10 +1185,13 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
     if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true, 1, 1, 2, 8>(stream, p) : launch_bf16_rows<false, 1, 1, 2, 8>(stream, p);
     const bool dma = reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && p.lda % 2 == 0 && p.K % 2 == 0 && p.K >= 8;   // A by DMA, or through registers
     const Bf16Tile tile = pick_bf16_tile(p);
-    if (!dma) {   // (A's way through registers bounds these: fewer forms)
+    if (!dma) {
+        // A's way through registers bounds these, and it is the shorter the more threads share a tile: 32 x 128 (1024 threads) in place of the middle sizes
+        // (256 x 4096 x 4095: 22 us, 64 x 128 tiles of 512 threads 48; 24 x 12288 x 4097: 16 x 64 17, 32 x 64 25)
         if (tile == BF16_128x256) return launch_bf16_tile<128, 256, 2, 4, 1, 3, false>(stream, p);
-        if (p.M > 32) return launch_bf16_tile<64, 128, 1, 4, 2, 3, false>(stream, p);
-        return tile == BF16_16x32 ? launch_bf16_tile<16, 32, 1, 2, 4, 3, false>(stream, p) : launch_bf16_tile<16, 64, 1, 4, 2, 3, false>(stream, p);
+        if (tile == BF16_16x32) return launch_bf16_tile<16, 32, 1, 2, 4, 3, false>(stream, p);
+        if (tile == BF16_16x64 || (tile == BF16_32x64 && p.M <= 32)) return launch_bf16_tile<16, 64, 1, 4, 2, 3, false>(stream, p);
+        return launch_bf16_tile<32, 128, 1, 4, 4, 2, false>(stream, p);
     }
     switch (tile) {
         case BF16_16x32: return launch_bf16_tile<16, 32, 1, 2, 4, 3, true>(stream, p);

@@ -312,6 +312,15 @@ def test_more_outputs_than_a_launch_holds(ctx, flux2mi, kind, m, n):
     assert torch.equal(out, av * wv[:, 0])
 
 
+@pytest.mark.parametrize("m,n,k", [(24, 12290, 131), (48, 2560, 261), (164, 1024, 3879), (100, 4100, 519), (300, 4200, 129), (600, 8000, 391)])
+def test_rows_of_odd_length(ctx, m, n, k):
+    """A in bf16 whose rows start in the middle of a dword, at every tile size."""
+    a, w, a64, w64 = operands(ctx, "bf16", m, n, k)
+    want, bound = R.gemm(a64, w64)
+    near(product(ctx, "bf16", a, w, dtype=torch.float32), want, bound, torch.float32)
+    near(product(ctx, "bf16", a, w), want, bound, torch.bfloat16)
+
+
 def test_column_slices_of_one_buffer(ctx):
     """Operands and results beside each other in the rows of one buffer share no element."""
     m, n, k = 37, 96, 160
