@@ -32,9 +32,9 @@ struct Range { uintptr_t lo, hi, pitch, width; };
 Range range_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t esz) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
     if (!p || rows <= 0 || cols <= 0) return Range{lo, lo, 0, 0};
-    uintptr_t last, hi;   // (no sizes wrap around: such a matrix reaches to the end of memory)
-    if (__builtin_mul_overflow((uintptr_t)(rows - 1), (uintptr_t)ld, &last) || __builtin_mul_overflow(last + (uintptr_t)cols, (uintptr_t)esz, &hi) ||
-        __builtin_add_overflow(lo, hi, &hi))
+    uintptr_t hi;   // (no sizes wrap around: such a matrix reaches to the end of memory)
+    if (__builtin_mul_overflow((uintptr_t)(rows - 1), (uintptr_t)ld, &hi) || __builtin_add_overflow(hi, (uintptr_t)cols, &hi) ||
+        __builtin_mul_overflow(hi, (uintptr_t)esz, &hi) || __builtin_add_overflow(lo, hi, &hi))
         hi = UINTPTR_MAX;
     return Range{lo, hi, (uintptr_t)ld * (uintptr_t)esz, (uintptr_t)cols * (uintptr_t)esz};
 }
@@ -45,8 +45,14 @@ bool overlap(const Range& a, const Range& b) {
     const uintptr_t d = b.lo > a.lo ? (b.lo - a.lo) % a.pitch : (a.pitch - (a.lo - b.lo) % a.pitch) % a.pitch;   // b's first column in a's rows
     return d < a.width || d + b.width > a.pitch;
 }
-Range codes_of(const void* p, int64_t rows, int64_t cols) { return range_of(p, 1, rows * (mxfp4_padded((int)cols) / 2), 0, 1); }
-Range scales_of(const void* p, int64_t rows, int64_t cols) { return range_of(p, 1, rows * (mxfp4_padded((int)cols) / 32), 0, 1); }
+Range codes_of(const void* p, int64_t rows, int64_t cols) { const int64_t row = mxfp4_padded((int)cols) / 2; return range_of(p, rows, row, row, 1); }
+Range scales_of(const void* p, int64_t rows, int64_t cols) { const int64_t row = mxfp4_padded((int)cols) / 32; return range_of(p, rows, row, row, 1); }
+// rows * (padded columns / values_per_byte), 0 for sizes that are none or do not fit 63 bits
+int64_t matrix_bytes(int64_t rows, int64_t cols, int values_per_byte) {
+    int64_t bytes;
+    if (rows < 0 || rows > MAX_ROWS || cols < 1 || cols > MAX_COLS || __builtin_mul_overflow(rows, (int64_t)(mxfp4_padded((int)cols) / values_per_byte), &bytes)) return 0;
+    return bytes;
+}
 
 int check_matrix(const char* who, const char* name, const uint8_t* codes, const uint8_t* scales) {
     F2_REQUIRE(codes && scales, FLUX2MI_ERR_INVALID_ARG, "%s: %s is NULL", who, name);
@@ -87,12 +93,8 @@ int run_gemm(const char* who, flux2mi_ctx* ctx, Mxfp4Gemm p, int out_dtype) {
 
 }  // namespace
 
-extern "C" int64_t flux2mi_mxfp4_code_bytes(int64_t rows, int64_t cols) {
-    return rows >= 0 && rows <= MAX_ROWS && cols >= 1 && cols <= MAX_COLS ? rows * (mxfp4_padded((int)cols) / 2) : 0;
-}
-extern "C" int64_t flux2mi_mxfp4_scale_bytes(int64_t rows, int64_t cols) {
-    return rows >= 0 && rows <= MAX_ROWS && cols >= 1 && cols <= MAX_COLS ? rows * (mxfp4_padded((int)cols) / 32) : 0;
-}
+extern "C" int64_t flux2mi_mxfp4_code_bytes(int64_t rows, int64_t cols) { return matrix_bytes(rows, cols, 2); }
+extern "C" int64_t flux2mi_mxfp4_scale_bytes(int64_t rows, int64_t cols) { return matrix_bytes(rows, cols, 32); }
 
 extern "C" int flux2mi_op_quantize_mxfp4(flux2mi_ctx* ctx, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* codes,
                                          uint8_t* scales) {

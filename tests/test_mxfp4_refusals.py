@@ -36,6 +36,17 @@ def test_sizes(lib):
     assert lib.flux2mi_mxfp4_code_bytes(1 << 33, 4096) == (1 << 33) * 2048   # past 32 bits
 
 
+@pytest.mark.parametrize("rows,cols", [((1 << 40) - 1, 1 << 30), (1 << 40, 1 << 30), (1 << 40, 1 << 26), (1 << 36, 1 << 28), ((1 << 33) + 1, 1 << 30), (1 << 33, 1 << 30)])
+def test_sizes_past_64_bits(lib, ctx, rows, cols):
+    """Sizes that do not fit 63 bits are 0, the largest that fit are right; a matrix of either reaches over every other buffer and is refused."""
+    for size, per_byte in ((lib.flux2mi_mxfp4_code_bytes, 2), (lib.flux2mi_mxfp4_scale_bytes, 32)):
+        want = rows * (cols // per_byte)
+        assert size(rows, cols) == (want if want < 1 << 63 else 0)
+    for x, codes, scales in ((A(0), A(1), A(2)), (A(2), A(1), A(0)), (A(1), A(0), A(2))):
+        refuses(lib, lib.flux2mi_op_quantize_mxfp4(ctx, x, F32, cols, rows, cols, codes, scales), INVALID, "overlap")
+        refuses(lib, lib.flux2mi_op_dequantize_mxfp4(ctx, codes, scales, rows, cols, x, BF16, cols), INVALID, "overlap")
+
+
 def refuses(lib, code, status, *words):
     assert code == status, (code, lib.flux2mi_last_error())
     if status != OK:
