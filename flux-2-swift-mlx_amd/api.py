@@ -634,13 +634,13 @@ class Context:
         """x' = resid_scale * x + gate * (norm_post(y) * post_weight);  out = norm(x') * weight * (1 + scale) + shift.
         x float32 [rows, dim], y bfloat16 / float32 or None; norms "none" | "rms" | "layer"; weights bfloat16 [dim]; gate, scale, shift
         float32 [dim], or a pair of them: the first for rows < split.  x' goes to x_out, by default into x itself.
-        -> (x', out): out of `dtype` (bfloat16 / float32), None without want_out."""
+        -> (x', out): out of `dtype` (bfloat16 / float32); without want_out None, and `norm` does not count."""
         x, ldx = self._matrix(x, (torch.float32,), "x", written=x_out is None)
         rows, dim = x.shape
         p = L.ResidualNorm(rows=rows, dim=dim, split=int(split), post_eps=post_eps, eps=eps, resid_scale=resid_scale, x=_ptr(x), ldx=ldx)
         if post_norm not in self._NORMS or norm not in self._NORMS:
             raise Flux2Error(L.ERR_INVALID_ARG, f"norms are {sorted(self._NORMS)}, got {post_norm!r}, {norm!r}")
-        p.post_norm, p.norm = self._NORMS[post_norm], self._NORMS[norm]
+        p.post_norm, p.norm = self._NORMS[post_norm], self._NORMS[norm] if want_out else L.NORM_NONE
         if y is not None:
             y, p.ldy = self._matrix(y, (torch.float32, torch.bfloat16), "y")
             if y.shape != x.shape:

@@ -89,6 +89,16 @@ def test_in_place_and_without_out(ctx):
         near(xd, xs, xerr, torch.float32)
 
 
+def test_without_out_by_default_norm(ctx):
+    """want_out=False with every other argument at its default: x' alone."""
+    x, y, _, _, _ = case(9, 640)
+    xs, xerr, _, _ = R.residual_norm(x, y)
+    xd = x.cuda()
+    _, none = ctx.op_residual_norm(xd, y.cuda(), want_out=False)
+    assert none is None
+    near(xd, xs, xerr, torch.float32)
+
+
 def test_strides(ctx):
     """x, y and x_out inside wider rows, aligned for vectors and not; what lies beside them stays."""
     for dim, c0, width in ((512, 4, 520), (512, 3, 520), (1029, 1, 1031)):
