@@ -566,7 +566,7 @@ class Context:
         return MXFP4(codes, scales, cols)
 
     def op_dequantize_mxfp4(self, m: MXFP4, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The values of `m` (exact in float32 and bfloat16)."""
+        """The values of `m` (exact in float32 and bfloat16, infinity from 2^128 on: scale bytes 253 and 254, which op_quantize_mxfp4 never writes)."""
         m = self._mxfp4(m, "m")
         if dtype not in _DT:
             raise Flux2Error(L.ERR_INVALID_ARG, f"dtype {dtype}")
@@ -620,7 +620,7 @@ class Context:
 
     def op_gemm_bf16_mxfp4(self, a: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
                            resid: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The same with a in bfloat16 [M, K]: only the weights are in 4 bits."""
+        """The same with a in bfloat16 [M, K]: only the weights are in 4 bits (an element of 2^128 or more counts as infinity here)."""
         a, lda = self._matrix(a, (torch.bfloat16,), "a")
         return self._gemm_mxfp4(lambda *r: lib().flux2mi_op_gemm_bf16_mxfp4(self.handle, _ptr(a), lda, *r),
                                 a.shape[0], a.shape[1], w, bias, gate, resid, dtype, out)

@@ -1,6 +1,7 @@
 // mxfp4_gemm.hip — products with MXFP4 weights (gfx950):  out = resid + gate * (A W^T + bias)
 //   A in MXFP4 (block scales ride in v_mfma_scale_f32_16x16x128_f8f6f4's scale operands) or in bf16 (W's codes become bf16 exactly, in
-//   registers: e2m1 x 2^e has 2 significant bits, then v_mfma_f32_16x16x32_bf16).
+//   registers: e2m1 x 2^e has 2 significant bits, down to the subnormal 2^-128; scale bytes 253 and 254, which the quantiser never writes, reach
+//   2^128 = infinity; then v_mfma_f32_16x16x32_bf16, which takes subnormals).
 // Every product of two code values is exact, sums are f32.
 //
 // Operand layout (both forms): lane l of a wave holds row l % 16 of its 16-row block and the 32 values 32 (l / 16) ... of a 128-value step:
@@ -23,7 +24,7 @@ __device__ __forceinline__ f32x4 mfma_fp4(u32x4 w, u32x4 a, f32x4 c, uint32_t sw
     const i32x8 wv = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0}, av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, c, 4, 4, 0, (int)sw, 0, (int)sa);
 }
-// 8 codes -> 8 bf16, exactly (the scale's exponent field alone is read: byte 0 is 2^-127, 255 NaN)
+// 8 codes -> 8 bf16, exactly below 2^128 (the scale's exponent field alone is read: byte 0 is 2^-127, 255 NaN)
 __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t q, float s) {
     u32x4 u;
     u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 0));

@@ -587,15 +587,17 @@ int flux2mi_op_attention_prescaled_range(flux2mi_ctx* ctx, const void* qkv, void
  *   byte = max(floor(log2 max|x|) - 2 + 127, 0), 0 for an all-zero block;  code = x / scale to the nearest value, ties to the even
  *   code, beyond 6 to +-6.  A block that holds a NaN or an infinity: byte 255, codes 0 — it reads back as NaN, and products with it are NaN.
  * Memory (device): codes u8 [rows][P / 2], two codes per byte, the even column in the low half; scales u8 [rows][P / 32]; P = cols
- * rounded up to a multiple of 128.  The padding is written as zeros, and a matrix from elsewhere must hold zeros there.  codes must
- * be 16-byte, scales 4-byte aligned.  Inputs and outputs of a call must not overlap unless said otherwise; rows, M or N of 0 do
+ * rounded up to a multiple of 128.  The padding is written as zeros, and a matrix from elsewhere must hold zeros there.  Scale bytes
+ * run up to 252 here; one from elsewhere may hold 253 and 254, whose elements of 2^128 or more (codes of 4 and 6; of 2 and more) are
+ * infinity wherever an element becomes f32 or bf16: read back, and in op_gemm_bf16_mxfp4.  op_gemm_mxfp4 multiplies them as they are.
+ * codes must be 16-byte, scales 4-byte aligned.  Inputs and outputs of a call must not overlap unless said otherwise; rows, M or N of 0 do
  * nothing.  All calls are async on the context's stream, allocate nothing and may be captured into a graph. */
 int64_t flux2mi_mxfp4_code_bytes(int64_t rows, int64_t cols);     /* rows * P / 2; 0 for invalid sizes */
 int64_t flux2mi_mxfp4_scale_bytes(int64_t rows, int64_t cols);    /* rows * P / 32 */
 /* x [rows, cols] of dtype f32 / bf16 / f16, row stride ldx elements -> codes, scales.  Exact: one rounding per value. */
 int flux2mi_op_quantize_mxfp4(flux2mi_ctx* ctx, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* codes,
                               uint8_t* scales);
-/* the values the codes stand for: exact in f32 and bf16, rounded once to f16 */
+/* the values the codes stand for: exact in f32 and bf16 (infinity from 2^128 on), rounded once to f16 */
 int flux2mi_op_dequantize_mxfp4(flux2mi_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y,
                                 int dtype, int64_t ldy);
 /* out [M, N] = resid + gate * (A W^T + bias): A [M, K] and W [N, K] in MXFP4, v_mfma_scale_f32_16x16x128_f8f6f4, f32 sums.
@@ -604,7 +606,8 @@ int flux2mi_op_dequantize_mxfp4(flux2mi_ctx* ctx, const uint8_t* codes, const ui
 int flux2mi_op_gemm_mxfp4(flux2mi_ctx* ctx, const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
                           const float* bias, const float* gate, const float* resid, int64_t ld_resid, void* out, int out_dtype,
                           int64_t ld_out, int M, int N, int K);
-/* the same with A in bf16 [M, K], row stride lda: only the weights are in 4 bits (they become bf16 exactly, in registers) */
+/* the same with A in bf16 [M, K], row stride lda: only the weights are in 4 bits (they become bf16 in registers: exactly, subnormals
+ * included; infinity from 2^128 on) */
 int flux2mi_op_gemm_bf16_mxfp4(flux2mi_ctx* ctx, const void* a, int64_t lda, const uint8_t* w, const uint8_t* w_scales,
                                const float* bias, const float* gate, const float* resid, int64_t ld_resid, void* out, int out_dtype,
                                int64_t ld_out, int M, int N, int K);
