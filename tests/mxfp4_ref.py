@@ -116,3 +116,51 @@ def residual_norm(x, y=None, split=0, post_norm="none", post_weight=None, post_e
         per = (xerr + rms) / sigma + n.abs() * rms / sigma
     oerr = f.abs() * (per + u64 * ((ROUNDINGS if norm != "none" else 4) * n.abs() + ROUNDINGS * spread * (norm == "layer"))) + 4 * u64 * (out.abs() + (f * n).abs())
     return xs, xerr, out, oerr
+
+
+def exact_operands(m: int, n: int, k: int, seed: int):
+    """Operands whose sums are exact in float32 in whatever order they are taken: (a, w), each (codes, scales) as numpy arrays.  Codes are random,
+    scales 2^-2 ... 2^1 and different in neighbouring blocks, so every product is a multiple of UNIT = (0.5 x 2^-2)^2 = 2^-6, and a sum of any of
+    them is exact while sum |a w| < 2^24 UNIT (24-bit significands)."""
+    rng = np.random.default_rng(seed)
+
+    def matrix(rows):
+        codes = rng.integers(0, 256, (rows, padded(k) // 2), dtype=np.uint8)
+        codes[:, (k + 1) // 2:] = 0
+        if k % 2:
+            codes[:, k // 2] &= 15
+        blocks = padded(k) // 32
+        step = rng.integers(1, 4, (rows, blocks))
+        step[:, 0] = rng.integers(0, 4, rows)
+        scales = (125 + np.cumsum(step, axis=1) % 4).astype(np.uint8)
+        scales[:, -(-k // 32):] = 0   # the padding
+        return codes, scales
+
+    return matrix(m), matrix(n)
+
+
+UNIT = 2.0 ** -6
+
+
+def exact_epilogue(m: int, n: int, seed: int):
+    """(bias, gate, resid): multiples of UNIT and powers of two, so that the epilogue is exact as well."""
+    g = torch.Generator().manual_seed(seed)
+    bias = torch.randint(-4096, 4097, (n,), generator=g) * UNIT
+    gate = torch.tensor([0.5, -1.0, 1.0, -0.5])[torch.randint(0, 4, (n,), generator=g)]
+    return bias, gate, torch.randint(-4096, 4097, (m, n), generator=g) * UNIT
+
+
+def exact_gemm(a64: torch.Tensor, w64: torch.Tensor, bias=None, gate=None, resid=None) -> torch.Tensor:
+    """float64 resid + gate (a w^T + bias), which is also what float32 gives: sum |a w| <= ||a|| ||w|| (taken itself where that is too wide); bias and
+    residual are at most 64 = 4096 UNIT, and a gate of 0.5 halves value and unit alike: (0.5 (sum + 64) + 64) / (UNIT / 2) = (sum + 192) / UNIT < 2^24."""
+    fits = lambda top: float(top) + 192 < 2.0 ** 24 * UNIT  # noqa: E731
+    assert fits(a64.norm(dim=1).max() * w64.norm(dim=1).max()) or fits((a64.abs() @ w64.abs().t()).max())
+    s = a64 @ w64.t()
+    if bias is not None:
+        s = s + bias.double()
+    if gate is not None:
+        s = s * gate.double()
+    if resid is not None:
+        s = s + resid.double()
+    assert torch.equal(s.float().double(), s)
+    return s

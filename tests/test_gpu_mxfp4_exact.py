@@ -1,0 +1,42 @@
+"""-m gpu: the two products on operands whose sums are exact in float32 (tests/mxfp4_ref.py, exact_operands): float32 results are the definition's
+bit for bit, bfloat16 results its one rounding.  Nothing of a sum can be lost, taken twice, scaled by another block's power of two or rounded on
+the way without showing.  Sizes are chosen by the kernel that the launch rules send them to, named beside them; the K are long enough for the
+steady state of each loop (16 scale bytes a row are 4 steps of 128, a ring's scales 16 steps)."""
+import pytest
+import torch
+
+from tests import mxfp4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def check(ctx, flux2mi, kind, m, n, k, lda=None, first_column=0):
+    """Plain and with the whole epilogue, both output types."""
+    from flux2mi.api import MXFP4
+    a, w = R.exact_operands(m, n, k, seed=m * 31 + n * 7 + k)
+    a64, w64 = R.dequantize(*a, k), R.dequantize(*w, k)
+    dev = lambda pair: MXFP4(torch.from_numpy(pair[0]).cuda(), torch.from_numpy(pair[1]).cuda(), k)  # noqa: E731
+    w4 = dev(w)
+    if kind == "mxfp4":
+        a4 = dev(a)
+        call = lambda **more: ctx.op_gemm_mxfp4(a4, w4, **more).cpu()  # noqa: E731
+    else:
+        if lda is None:
+            ab = a64.bfloat16().cuda()
+        else:   # inside wider rows, NaN around
+            ab = torch.full((m * lda + first_column,), float("nan"), dtype=torch.bfloat16, device="cuda").as_strided((m, k), (lda, 1), first_column)
+            ab.copy_(a64.bfloat16())
+        call = lambda **more: ctx.op_gemm_bf16_mxfp4(ab, w4, **more).cpu()  # noqa: E731
+    bias, gate, resid = R.exact_epilogue(m, n, m + n)
+    want = R.exact_gemm(a64, w64)
+    assert torch.equal(call(dtype=torch.float32).double(), want)
+    assert torch.equal(call(dtype=torch.bfloat16), want.float().bfloat16())
+    want = (want + bias.double()) * gate.double()
+    assert torch.equal(call(bias=bias.cuda(), gate=gate.cuda(), dtype=torch.bfloat16), want.float().bfloat16())
+    assert torch.equal(call(bias=bias.cuda(), gate=gate.cuda(), resid=resid.cuda()).double(), want + resid.double())
+
+
+@pytest.mark.parametrize("m,n", [(1100, 12288), (700, 2500)])   # 256 x 256 tiles, 128 x 128 tiles
+@pytest.mark.parametrize("k", [2049, 2200, 2400, 2560])         # 17, 18, 19 and 20 steps: every remainder of a last group of four
+def test_mxfp4_tiles_in_their_steady_state(ctx, flux2mi, m, n, k):
+    check(ctx, flux2mi, "mxfp4", m, n, k)
