@@ -40,3 +40,10 @@ def check(ctx, flux2mi, kind, m, n, k, lda=None, first_column=0):
 @pytest.mark.parametrize("k", [2049, 2200, 2400, 2560])         # 17, 18, 19 and 20 steps: every remainder of a last group of four
 def test_mxfp4_tiles_in_their_steady_state(ctx, flux2mi, m, n, k):
     check(ctx, flux2mi, "mxfp4", m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(4500, 4100, 1700), (4500, 4104, 2047), (4500, 4100, 2300), (4500, 4104, 2420)])   # 14, 16, 18 and 19 steps
+def test_mxfp4_columns_split_over_two_launches(ctx, flux2mi, m, n, k):
+    """18 x 17 large tiles are 1.2 rounds of 256: 14 columns of them are launched as they are, the others as 128 x 128 tiles, and w, its scales, bias, gate,
+    resid and out move along (4104 columns: 16-byte rows of bfloat16 as well).  The first launch alone would cost two rounds, the second alone 2.3."""
+    check(ctx, flux2mi, "mxfp4", m, n, k)
