@@ -47,3 +47,24 @@ def test_mxfp4_columns_split_over_two_launches(ctx, flux2mi, m, n, k):
     """18 x 17 large tiles are 1.2 rounds of 256: 14 columns of them are launched as they are, the others as 128 x 128 tiles, and w, its scales, bias, gate,
     resid and out move along (4104 columns: 16-byte rows of bfloat16 as well).  The first launch alone would cost two rounds, the second alone 2.3."""
     check(ctx, flux2mi, "mxfp4", m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(7, 4000, 2570), (4, 9000, 3001),                                  # 16-row workgroups
+                                   (13, 5003, 6660), (64, 4096, 4226), (40, 2500, 16000),             # 16 x 64 tiles, four k groups
+                                   (30, 12290, 4300), (128, 4096, 5000),                              # 32 x 64
+                                   (100, 5120, 4400), (250, 3000, 4480), (190, 4100, 2050)])          # 32 x 128
+def test_mxfp4_few_rows(ctx, flux2mi, m, n, k):
+    check(ctx, flux2mi, "mxfp4", m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 3000), (5, 300, 4400), (23, 5121, 5120), (48, 2560, 2600), (40, 2500, 16000),   # A whole in LDS; 16 x 32 tiles
+                                   (64, 4096, 2100), (100, 4100, 2600),                               # 16 x 64
+                                   (30, 12290, 4300), (128, 4096, 2562),                              # 32 x 64
+                                   (100, 5120, 4400), (256, 4096, 2560),                              # 32 x 128
+                                   (250, 6000, 2600), (512, 4096, 2700),                              # 64 x 128
+                                   (300, 12288, 1030), (4500, 4100, 1700),                            # 64 x 256
+                                   (600, 8000, 1300), (1100, 12288, 1300),                            # 128 x 256
+                                   (48, 2560, 2601), (164, 1024, 3879), (24, 12290, 2049), (24, 5120, 2049),   # rows of odd length: 16 x 32, 16 x 64
+                                   (300, 4200, 1029), (700, 2500, 2049), (600, 8000, 1291)])          # 32 x 128, 128 x 256
+def test_bf16_tiles(ctx, flux2mi, m, n, k):
+    check(ctx, flux2mi, "bf16", m, n, k)
