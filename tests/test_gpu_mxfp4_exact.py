@@ -68,3 +68,10 @@ def test_mxfp4_few_rows(ctx, flux2mi, m, n, k):
                                    (300, 4200, 1029), (700, 2500, 2049), (600, 8000, 1291)])          # 32 x 128, 128 x 256
 def test_bf16_tiles(ctx, flux2mi, m, n, k):
     check(ctx, flux2mi, "bf16", m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 200, 9000), (4, 200, 8192), (4, 200, 8193), (4, 37, 20001), (3, 200, 12001), (3, 200, 10242), (2, 200, 17000), (2, 33, 16385), (1, 40, 33000)])
+def test_bf16_rows_in_several_chunks(ctx, flux2mi, m, n, k):
+    """Up to 4 rows: 64 KB of A in LDS at a time (8192 k of 4 rows, 10240 of 3, 16384 of 2, 32768 of one), staged anew while W streams on; the rows of
+    odd length are staged through shifted dwords."""
+    check(ctx, flux2mi, "bf16", m, n, k)
