@@ -75,3 +75,46 @@ def test_bf16_rows_in_several_chunks(ctx, flux2mi, m, n, k):
     """Up to 4 rows: 64 KB of A in LDS at a time (8192 k of 4 rows, 10240 of 3, 16384 of 2, 32768 of one), staged anew while W streams on; the rows of
     odd length are staged through shifted dwords."""
     check(ctx, flux2mi, "bf16", m, n, k)
+
+
+@pytest.mark.parametrize("lda,first_column", [(1 << 24, 0), (1 << 24, 8), ((1 << 24) + 8, 3), ((1 << 24) + 1, 0), ((1 << 24) - 8, 8), ((1 << 24) - 1, 1)])
+@pytest.mark.parametrize("m,n,k", [(5, 70, 200), (40, 300, 2300), (33, 130, 1001)])
+def test_bf16_rows_far_apart(ctx, flux2mi, m, n, k, lda, first_column):
+    """Rows of A 2^24 elements apart leave the 32-bit offsets of the tiles: 16 rows a workgroup, A in 64 KB chunks, whole and from an odd column on; just
+    below that stride the tiles take them."""
+    check(ctx, flux2mi, "bf16", m, n, k, lda=lda, first_column=first_column)
+
+
+@pytest.mark.parametrize("k", [(1 << 24) - 2, 1 << 24, (1 << 24) + 130])
+@pytest.mark.parametrize("kind", ["mxfp4", "bf16"])
+def test_k_past_the_tiles_offsets(ctx, flux2mi, kind, k):
+    """K on both sides of 2^24, more rows than a 16-row workgroup has: operands that are zero but for some columns, the first and the last among them."""
+    from flux2mi.api import MXFP4
+    m, n = 21, 35
+    at = torch.tensor([0, 1, 127, 128, 8191, 8192, 65537, 1 << 20, (1 << 23) + 77, k - 129, k - 2, k - 1])
+    g = torch.Generator().manual_seed(k)
+    codes = lambda rows: torch.randint(0, 16, (rows, len(at)), generator=g)  # noqa: E731
+    ac, wc, p = codes(m), codes(n), R.padded(k)
+
+    def matrix(c):
+        q, s = torch.zeros((len(c), p // 2), dtype=torch.uint8, device="cuda"), torch.zeros((len(c), p // 32), dtype=torch.uint8, device="cuda")
+        for j, column in enumerate(at.tolist()):
+            q[:, column // 2] |= (c[:, j] << (4 * (column & 1))).to(torch.uint8).cuda()
+            s[:, column // 32] = 126 + column % 3
+        return MXFP4(q, s, k)
+
+    table = torch.from_numpy(R.E2M1)
+    value = lambda c: torch.where(c >= 8, -1.0, 1.0) * table[c & 7]  # noqa: E731
+    scale = {}   # columns of one block share the last one's
+    for column in at.tolist():
+        scale[column // 32] = 2.0 ** (column % 3 - 1)
+    scale = torch.tensor([scale[column // 32] for column in at.tolist()], dtype=torch.float64)
+    a64, w64 = value(ac) * scale, value(wc) * scale
+    w4 = matrix(wc)
+    if kind == "mxfp4":
+        got = ctx.op_gemm_mxfp4(matrix(ac), w4, dtype=torch.float32)
+    else:
+        a = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+        a[:, at.cuda()] = a64.bfloat16().cuda()
+        got = ctx.op_gemm_bf16_mxfp4(a, w4, dtype=torch.float32)
+    assert torch.equal(got.double().cpu(), a64 @ w64.t())   # multiples of 2^-4 below 2^14: exact in float32
