@@ -9,7 +9,11 @@
     * exactly the instruction mix the schedule tables describe (MFMA / ds_read / DMA counts per trip)
   and the kernels use no scratch at all; in particular no block that issues an MFMA may touch scratch: a spill store of an accumulator
   placed behind the asm MFMA that writes it stores a register whose result is still in flight.
-Part of the product build: csrc/Makefile compiles the three objects with -save-temps=obj and runs `check_isa.py --from build` on the
+
+  mxfp4_gemm.hip's tile kernel keeps its MFMAs in asm too (check_mxfp4_tile below): accumulators stay in place, no copy and no scratch between the
+  first and the last MFMA of a trip, no VALU result read by an MFMA within the wait states that hipcc does not count for asm, M0 kept from a
+  DMA piece to the three that share it, the vmcnt of the two hand-overs and no other, accumulators read behind the drain.
+Part of the product build: csrc/Makefile compiles the objects with -save-temps=obj and runs `check_isa.py --from build` on the
 device assembly OF THE OBJECTS THAT ARE LINKED (build/isa.ok is a prerequisite of libflux2mi.so), so a toolchain bump or a source edit
 that breaks an invariant fails the build; tests/test_isa_invariants.py re-runs it on the same files.  Stand-alone (compiles its own
 assembly, ~5 min): python tools/check_isa.py"""
@@ -32,7 +36,8 @@ def compile_s(name):
         return open(os.path.join(FROM, name + "-hip-amdgcn-amd-amdhsa-gfx950.s")).read()
     os.makedirs(OUT, exist_ok=True)
     dst = os.path.join(OUT, name + ".s")
-    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-w", "-S", "--offload-device-only",
+    unpacked = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if name.startswith("mxfp4") else []   # as csrc/Makefile builds them
+    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-w", *unpacked, "-S", "--offload-device-only",
                     os.path.join(CSRC, name + ".hip"), "-o", dst], check=True)
     return open(dst).read()
 
@@ -91,6 +96,95 @@ def check_m0(name, text, errors):
     print(f"{name}: M0 references besides the LDS-DMA setup: {len(bad)}")
     if bad:
         errors.append((name, "foreign M0 references", bad[:5]))
+
+
+def registers(operand):
+    """{(file, number)} of "v7", "a[12:15]"; empty for anything else"""
+    m = re.fullmatch(r"([va])(?:(\d+)|\[(\d+):(\d+)\])", operand.strip())
+    return {(m.group(1), i) for i in range(int(m.group(2) or m.group(3)), int(m.group(2) or m.group(4)) + 1)} if m else set()
+
+
+def operands(ins):
+    return [o.strip() for o in ins.split(None, 1)[1].split(" op_sel")[0].split(",")] if " " in ins else []
+
+
+MFMA_WAIT_STATES = 4   # between a VALU write and an MFMA that reads it (the hardware asks for 2; hipcc counts none for asm)
+
+
+def check_mxfp4_tile(text, errors):
+    """mxfp4_gemm_tile_kernel<BM, BN, ., ., CUT, .>: MT x NT MFMAs a phase, four phases a trip; NP code pieces per stage, two stages a trip."""
+    found = 0
+    for kname, body in kernels(text):
+        m = re.search(r"\d+mxfp4_gemm_tile_kernelILi(\d+)ELi(\d+)ELb(\d)ELb(\d)ELi(\d)ELi\d+E", kname)
+        if not m or "bf16_mxfp4" in kname:
+            continue
+        found += 1
+        bm, bn, cut = int(m.group(1)), int(m.group(2)), int(m.group(5))
+        mt, nt, slots, np_, sr = bm // 32, bn // 32, bm * bn // 1024, (bm + bn) // 32, (bm + bn) // 256
+        free, every = slots // 2, slots * 3 // 2 // np_
+        flying = (slots - free - 2) // every + 1
+        short = cut == 2
+        wrong = []
+        scratch, spills = meta(text, kname, "private_segment_fixed_size"), meta(text, kname, "vgpr_spill_count")
+        if scratch or spills:
+            wrong.append(f"scratch {scratch} B, spills {spills}")
+        loops = [(label, ins) for label, ins in blocks(body) if sum(i.startswith("v_mfma") for i in ins) == 4 * slots]
+        if len(loops) != 1 or sum(i.split(";")[0].strip().startswith("v_mfma") for i in body.split("\n")) != 4 * slots:
+            errors.append((kname, "the loop of four phases was not found, or there are MFMAs outside"))
+            continue
+        label, ins = loops[0]
+        op = [i.split()[0] for i in ins]
+        c = collections.Counter(op)
+        mfma = [k for k, o in enumerate(op) if o.startswith("v_mfma")]
+        want = {"ds_read_b128": 4 * (mt + nt) + (mt + nt) // 4 + (0 if short else sr), "global_load_lds_dwordx4": 2 * np_ + (0 if short else 2 * sr),
+                "global_load_lds_dword": 4 * sr if short else 0, "s_barrier": 4}
+        wrong += [f"{c.get(o, 0)} {o}, not {n}" for o, n in want.items() if c.get(o, 0) != n]
+        wrong += [i for i in ins if i.startswith(("v_accvgpr", "scratch_", "buffer_", "flat_", "global_")) and not i.startswith("global_load_lds_dword")]
+        wrong += ["copy: " + i for i in ins[mfma[0]:mfma[-1]] if i.startswith("v_mov") and re.search(r",\s*[va]\[?\d", i)]
+        waits = [i for i in ins if i.startswith("s_waitcnt") and "vmcnt" in i]
+        if waits != [f"s_waitcnt vmcnt({flying}) lgkmcnt(0)"] * 2:
+            wrong.append(f"vmcnt waits {waits}")
+        accumulators = collections.Counter()
+        for k in mfma:
+            o = operands(ins[k])
+            if o[0] != o[3] or not o[0].startswith("a["):
+                wrong.append("accumulator moves: " + ins[k])
+            accumulators[o[0]] += 1
+        if len(accumulators) != slots or set(accumulators.values()) != {4}:
+            wrong.append(f"{len(accumulators)} accumulators")
+        # VALU write -> MFMA read, over the back edge too (a VALU result never is an accumulator's: v_accvgpr is refused above)
+        twice = ins + ins
+        for k, i in enumerate(ins):
+            if not i.startswith("v_") or i.startswith(("v_mfma", "v_cmp")):
+                continue
+            written, states = registers(operands(i)[0]), 0
+            for j in twice[k + 1:]:
+                if states >= MFMA_WAIT_STATES:
+                    break
+                if j.startswith("v_mfma") and any(written & registers(o) for o in operands(j)):
+                    wrong.append(f"{i}  read {states} wait states on by  {j}")
+                states += int(j.split()[1], 0) + 1 if j.startswith("s_nop") else 1
+        # M0: a piece with an offset shares the M0 of the piece before it that set M0 in front of its MFMA (and follows it without another write)
+        owner = None
+        for k, i in enumerate(ins):
+            if re.search(r"\bm0\b", i):
+                if not re.match(r"s_mov_b32 m0, s\d+$", i):
+                    wrong.append("M0: " + i)
+                owner = "piece" if op[k + 1].startswith("v_mfma") else "scales"
+            elif op[k] == "global_load_lds_dwordx4" and " offset:" in i and owner != "piece":
+                wrong.append("M0 is not this piece's: " + i)
+        # behind the loop: two s_nop 15 in front of the first accumulator read
+        behind = [l.split(";")[0].strip() for l in body.split(ins[-1], 1)[1].split("\n")]
+        behind = [l for l in behind if l and not l.startswith(".")]
+        first = next((k for k, l in enumerate(behind) if l.startswith("v_accvgpr_read") or re.search(r"\ba\[?\d", l)), len(behind))
+        if sum(l == "s_nop 15" for l in behind[:first]) < 2:
+            wrong.append("accumulators are read before they have drained")
+        print(f"mxfp4_gemm_tile_kernel<{', '.join(m.groups())}>: scratch {scratch} B; {label}: {len(ins)} instructions, {len(mfma)} MFMA, {c['ds_read_b128']} ds_read_b128, "
+              f"{c['global_load_lds_dwordx4']} LDS-DMA  {'VIOLATION' if wrong else 'ok'}")
+        if wrong:
+            errors.append((kname, label, *wrong))
+    if not found:
+        errors.append(("mxfp4_gemm", "no mxfp4_gemm_tile_kernel found"))
 
 
 def main():
@@ -160,6 +254,10 @@ def main():
                 found = True
         if not found:
             errors.append((kname, "three-tile loop not found"))
+    # ---- MXFP4 x MXFP4 tiles
+    text = compile_s("mxfp4_gemm")
+    check_m0("mxfp4_gemm", text, errors)
+    check_mxfp4_tile(text, errors)
     if errors:
         print("FAILED:", *errors, sep="\n  ")
         sys.exit(1)
