@@ -502,6 +502,9 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
         // the scales of groups q + 2 and q + 3 (q even) are requested in P1 and have landed at the hand-over behind P2; P3 transposes those of group q + 2
         // and reads those of group q + 1
         u32x4 raw[SR], next[(NT + MT) / 4];
+#pragma unroll
+        for (int t = 0; t < (NT + MT) / 4; ++t) asm volatile("" : "+v"(sc[t]));
+        asm volatile("s_nop 7" ::: "memory");   // the copies of `next` into the scale registers have settled
         auto phase = [&](auto op) {
             constexpr int OP = decltype(op)::value, CUR = OP & 1, NBUF = OP == 1 || OP == 2 ? 1 : 0, NKS = OP & 1 ? 0 : 1;
             constexpr int READS = MT + NT, RSPAN = OP & 1 ? SLOTS / 2 : SLOTS * 3 / 8;
@@ -551,7 +554,6 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
         lds_returned();
 #pragma unroll
         for (int t = 0; t < (NT + MT) / 4; ++t) sc[t] = next[t];
-        asm volatile("s_nop 7" ::: "memory");   // (a copy of a scale register, if there is one, settles)
     }
     drain<MT, NT>(acc);
     hand_over<0>();   // everybody has left the stages: their LDS becomes the epilogue's

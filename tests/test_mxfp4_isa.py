@@ -69,6 +69,7 @@ def sources(text, n):
     ("vmcnt", lambda t: behind_mfma(t, 90, "s_waitcnt vmcnt(0)")),
     ("wait states", lambda t: behind_mfma(t, 99, f"v_add_u32_e32 {sources(t, 101)[4]}, 1, v250")),
     ("wait states", lambda t: behind_mfma(t, 98, f"v_lshlrev_b32_e32 v{re.search('[0-9]+', sources(t, 100)[1]).group(0)}, 1, v250")),
+    ("behind the copies", lambda t: t.replace("s_nop 7", "s_nop 0")),
     ("accumulator moves", lambda t: t.replace(re.findall(r"^\tv_mfma.*$", t, re.M)[9], "\tv_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[2:5], v[6:9], a[4:7], v10, v11 op_sel_hi:[0,0,0] cbsz:4 blgp:4", 1)),
     ("ds_read_b128", lambda t: behind_mfma(t, 30, "ds_read_b128 v[250:253], v249")),
     ("drained", lambda t: t.replace("s_nop 15", "s_nop 0")),

@@ -164,6 +164,11 @@ def check_mxfp4_tile(text, errors):
                 if j.startswith("v_mfma") and any(written & registers(o) for o in operands(j)):
                     wrong.append(f"{i}  read {states} wait states on by  {j}")
                 states += int(j.split()[1], 0) + 1 if j.startswith("s_nop") else 1
+        # the scale registers of the next trip are copied behind the last MFMA: an s_nop 7 of the kernel's own stands between them and the first one
+        between = ins[mfma[-1] + 1:] + ins[:mfma[0]]
+        copies = [k for k, i in enumerate(between) if i.startswith("v_mov") and re.search(r",\s*[va]\[?\d", i)]
+        if copies and "s_nop 7" not in between[copies[-1]:]:
+            wrong.append("no s_nop 7 behind the copies of the scale registers")
         # M0: a piece with an offset shares the M0 of the piece before it that set M0 in front of its MFMA (and follows it without another write)
         owner = None
         for k, i in enumerate(ins):
