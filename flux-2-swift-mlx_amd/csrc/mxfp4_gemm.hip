@@ -82,11 +82,13 @@ __device__ __forceinline__ bf16x8 load_a8(const uint16_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------------------------------------- few rows: K split over the waves of a workgroup
-// 16 rows x 16 columns per workgroup; its WAVES waves take the 128-value steps in turn (so that together they read whole lines of W) and
+// 16 rows x 16 columns per workgroup; its waves take the 128-value steps in turn (so that together they read whole lines of W) and
 // their sums are added in wave order through LDS.  Bound by latency (8 x 2560 x 2560: 3.6 us) and, with more columns, by reading W: operands go straight
 // from memory to registers, U steps of a wave at a time, and the next U are requested before the current ones are used.
-template <bool VEC, int U, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n) {
+constexpr int ROWS_WAVES = 4;
+template <bool VEC>
+__global__ __launch_bounds__(64 * ROWS_WAVES) void mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n) {
+    constexpr int U = 4, WAVES = ROWS_WAVES;
     __shared__ f32x4 part[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16, steps = p.steps;
@@ -683,32 +685,25 @@ bool wide_rows(const Mxfp4Gemm& p) {
     return p.N % cols == 0 && ok(p.out, p.ld_out, cols) && ok(p.resid, p.ld_resid, 4) && ok(p.bias, 0, 4) && ok(p.gate, 0, 4);
 }
 // ---------------------------------------------------------------------------------------------- the same with A in bf16
-// A is shared by every wave of a workgroup and comes once per workgroup through LDS, `chunk` steps of all its rows at a time (chunk % WAVES == 0, so
+// A is shared by every wave of a workgroup and comes once per workgroup through LDS, `chunk` steps of all its rows at a time (a multiple of the waves' U steps, so
 // that a wave's steps wave, wave + WAVES, ... fall into the chunks alike); W and its scales stream through registers across the chunks.
 // Read by every wave for itself, A costs four loads per step against one of W: the vector-memory path, not HBM, is then the bound.
 // Measured: 1 x 19456 x 2560 8.6 us = 3.1 TB/s of W; bound by the latency of staging A and of a wave's first loads.
-template <bool AVEC, bool VEC, int MT, int NT, int U, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n, int chunk) {
-    extern __shared__ __align__(16) uint8_t smem[];   // A: [rows][chunk * 256 + 16] bytes; then the partial sums [WAVES][MT * NT][64]
+constexpr int BF16_ROWS_U = 2, BF16_ROWS_WAVES = 8;
+template <bool AVEC, bool VEC>
+__global__ __launch_bounds__(64 * BF16_ROWS_WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n, int chunk) {
+    constexpr int U = BF16_ROWS_U, WAVES = BF16_ROWS_WAVES;
+    extern __shared__ __align__(16) uint8_t smem[];   // A: [rows][chunk * 256 + 16] bytes; then the partial sums [WAVES][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n0 = (int)(blockIdx.x % tiles_n) * 16 * NT, m0 = (int)(blockIdx.x / tiles_n) * 16 * MT;
-    const int64_t row_bytes = (int64_t)p.steps * 64, row_scales = (int64_t)p.steps * 4;
-    const int steps = p.steps, rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT, pitch = chunk * 256 + 16;
-    const uint8_t *wq[NT], *ws[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {   // rows behind the last one: its copy, never stored
-        const int64_t n = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
-        wq[j] = p.w + n * row_bytes + g * 16;
-        ws[j] = p.w_scales + n * row_scales + g;
-    }
-    struct Step { u32x4 w[NT]; uint32_t s[NT]; };
+    const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16;
+    const int steps = p.steps, rows = p.M - m0 < 16 ? p.M - m0 : 16, pitch = chunk * 256 + 16;
+    const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;   // rows behind the last one: its copy, never stored
+    const uint8_t *wq = p.w + n * steps * 64 + g * 16, *ws = p.w_scales + n * steps * 4 + g;
+    struct Step { u32x4 w; uint32_t s; };
     auto load = [&](int s, Step& x) {
         if (s >= steps) return;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            x.w[j] = *reinterpret_cast<const u32x4*>(wq[j] + (int64_t)s * 64);
-            x.s[j] = ws[j][(int64_t)s * 4];
-        }
+        x.w = *reinterpret_cast<const u32x4*>(wq + (int64_t)s * 64);
+        x.s = ws[(int64_t)s * 4];
     };
     const uint16_t* a = reinterpret_cast<const uint16_t*>(p.a);
     auto stage = [&](int first) {   // steps first ... first + chunk - 1 of A; columns >= K are zero
@@ -718,27 +713,15 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
             if (k < steps * 128) *reinterpret_cast<bf16x8*>(smem + row * pitch + c * 16) = load_a8<AVEC>(a + (int64_t)(m0 + row) * p.lda, k, p.K);
         }
     };
-    const uint8_t* arow[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) arow[i] = smem + (16 * i + r < rows ? 16 * i + r : rows - 1) * pitch + g * 64;
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t* arow = smem + (r < rows ? r : rows - 1) * pitch + g * 64;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     auto use = [&](int s, int first, const Step& x) {
         if (s >= steps) return;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            bf16x8 b[MT];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) b[i] = *reinterpret_cast<const bf16x8*>(arow[i] + (s - first) * 256 + q * 16);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const bf16x8 w = codes_to_bf16(x.w[j][q], __builtin_bit_cast(float, x.s[j] << 23));
-#pragma unroll
-                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, b[i], acc[j][i], 0, 0, 0);
-            }
+            const bf16x8 b = *reinterpret_cast<const bf16x8*>(arow + (s - first) * 256 + q * 16);
+            const uint32_t code = x.w[q];
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(code, __builtin_bit_cast(float, x.s << 23)), b, acc, 0, 0, 0);
         }
     };
     Step cur[U], next[U];
@@ -759,18 +742,13 @@ __global__ __launch_bounds__(64 * WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4G
         }
     }
     __syncthreads();
-    f32x4* part = reinterpret_cast<f32x4*>(smem);   // [WAVES][MT * NT][64]
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) part[(wave * MT * NT + j * MT + i) * 64 + lane] = acc[j][i];
+    f32x4* part = reinterpret_cast<f32x4*>(smem);
+    part[wave * 64 + lane] = acc;
     __syncthreads();
-    for (int t = wave; t < MT * NT; t += WAVES) {
-        f32x4 v = part[t * 64 + lane];
+    if (wave) return;
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += part[(w * MT * NT + t) * 64 + lane];
-        store4<VEC>(p, m0 + 16 * (t % MT) + r, n0 + 16 * (t / MT) + 4 * g, v);
-    }
+    for (int w = 1; w < WAVES; ++w) acc += part[w * 64 + lane];
+    store4<VEC>(p, m0 + r, n0 + 4 * g, acc);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles staged through LDS (bf16 x MXFP4)
@@ -1002,30 +980,29 @@ bool four_columns(const Mxfp4Gemm& p) {
 }
 
 int launch_rows(hipStream_t stream, const Mxfp4Gemm& p) {
-    constexpr int U = 4, WAVES = 4;
     const int tn = (p.N + 15) / 16, tm = (p.M + 15) / 16;
-    const dim3 grid((unsigned)(tn * (int64_t)tm)), block(64 * WAVES);
-    if (four_columns(p)) mxfp4_gemm_rows_kernel<true, U, WAVES><<<grid, block, 0, stream>>>(p, tn);
-    else mxfp4_gemm_rows_kernel<false, U, WAVES><<<grid, block, 0, stream>>>(p, tn);
+    const dim3 grid((unsigned)(tn * (int64_t)tm)), block(64 * ROWS_WAVES);
+    if (four_columns(p)) mxfp4_gemm_rows_kernel<true><<<grid, block, 0, stream>>>(p, tn);
+    else mxfp4_gemm_rows_kernel<false><<<grid, block, 0, stream>>>(p, tn);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-template <bool AVEC, int MT, int NT, int U, int WAVES>
+template <bool AVEC>
 int launch_bf16_rows(hipStream_t stream, const Mxfp4Gemm& p) {
-    const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT);
-    const int rows = p.M < 16 * MT ? p.M : 16 * MT, unit = WAVES * U;
-    int chunk = 65536 / (rows * 256) / unit * unit;                    // A's part of LDS: 64 KB
-    if (chunk < unit) chunk = unit;
+    constexpr int unit = BF16_ROWS_WAVES * BF16_ROWS_U;
+    const int64_t tn = (p.N + 15) / 16, tm = (p.M + 15) / 16;
+    const int rows = p.M < 16 ? p.M : 16;
+    int chunk = 65536 / (rows * 256) / unit * unit;                    // A's part of LDS: 64 KB (at least one unit: 16 rows x 16 steps)
     const int all = (p.steps + unit - 1) / unit * unit;
     if (chunk > all) chunk = all;
-    const int lds_a = rows * (chunk * 256 + 16), lds_sums = WAVES * MT * NT * 1024, lds = lds_a > lds_sums ? lds_a : lds_sums;
-    const dim3 grid((unsigned)(tn * tm)), block(64 * WAVES);
-    const bool vec = four_columns(p);
-    const auto fn = vec ? bf16_mxfp4_gemm_rows_kernel<AVEC, true, MT, NT, U, WAVES> : bf16_mxfp4_gemm_rows_kernel<AVEC, false, MT, NT, U, WAVES>;
+    const int lds_a = rows * (chunk * 256 + 16), lds_sums = BF16_ROWS_WAVES * 1024, lds = lds_a > lds_sums ? lds_a : lds_sums;
+    const dim3 grid((unsigned)(tn * tm)), block(64 * BF16_ROWS_WAVES);
+    const auto fn = four_columns(p) ? bf16_mxfp4_gemm_rows_kernel<AVEC, true> : bf16_mxfp4_gemm_rows_kernel<AVEC, false>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return 2;
     fn<<<grid, block, lds, stream>>>(p, (int)tn, chunk);
     return hipGetLastError() == hipSuccess ? 0 : 2;
 }
+
 template <int BM, int BN, int PER_CU, bool BF16, bool VEC, int CUT>
 int launch_tile_form(hipStream_t stream, const Mxfp4Gemm& p) {
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
@@ -1185,7 +1162,7 @@ int launch_mxfp4_gemm(hipStream_t stream, const Mxfp4Gemm& p) {
     }
     const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % 8 == 0;
     // few rows: A whole in LDS (1 x 19456 x 2560 8.5 us, 16-row tiles 11; at 16 rows 23.7 against 8.7)
-    if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true, 1, 1, 2, 8>(stream, p) : launch_bf16_rows<false, 1, 1, 2, 8>(stream, p);
+    if (p.M <= 4 || !offsets32) return aligned ? launch_bf16_rows<true>(stream, p) : launch_bf16_rows<false>(stream, p);
     const bool dma = reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && p.lda % 2 == 0 && p.K % 2 == 0 && p.K >= 8;   // A by DMA, or through registers
     const Bf16Tile tile = pick_bf16_tile(p);
     if (!dma) {
