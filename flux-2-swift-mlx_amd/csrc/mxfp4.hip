@@ -6,8 +6,8 @@
 // ties to the even code, |x| / scale > 6 to +-6.  A block that holds a NaN or an infinity gets byte 255 (= NaN for its consumers) and zero codes.
 // All of it is exact: the division is by a power of two and v_cvt_scalef32_pk_fp4_f32 rounds once (subnormal inputs and scales included).
 //
-// Both kernels are bound by HBM: 36864 x 4096 f32 quantised in 122 us (5.6 TB/s; 158 right behind a pass that wrote 600 MB), read back in 121 to
-// 135; 512 x 2560 bf16 3 us each, a launch's latency.  One pass, 8 values per lane (a quad of lanes = one block, its maximum by two DPP steps, no LDS).
+// Both kernels are bound by HBM: 36864 x 4096 f32 quantised in 123 us (5.6 TB/s; 158 right behind a pass that wrote 600 MB), read back in 120 to
+// 132, bf16 66 and 69 us; 20000 x 5119 bf16 (every other row starts in the middle of a dword) 50 and 79 us; 512 x 2560 bf16 3 us each, a launch's latency.  One pass, 8 values per lane (a quad of lanes = one block, its maximum by two DPP steps, no LDS).
 // Rows may start at any element: whole dwords are moved all the same (a row of 2-byte values that starts in the middle of one is shifted in registers).
 #include "dev.h"
 #include "mxfp4.h"

@@ -83,7 +83,7 @@ __device__ __forceinline__ bf16x8 load_a8(const uint16_t* row, int k, int K) {
 
 // ---------------------------------------------------------------------------------------------- few rows: K split over the waves of a workgroup
 // 16 rows x 16 columns per workgroup; its waves take the 128-value steps in turn (so that together they read whole lines of W) and
-// their sums are added in wave order through LDS.  Bound by latency (8 x 2560 x 2560: 3.6 us) and, with more columns, by reading W: operands go straight
+// their sums are added in wave order through LDS.  Bound by latency (8 x 2560 x 2560: 3.6 us with W in the caches, 4.2 from HBM) and, with more columns, by reading W: operands go straight
 // from memory to registers, U steps of a wave at a time, and the next U are requested before the current ones are used.
 constexpr int ROWS_WAVES = 4;
 template <bool VEC>
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mxfp4_gemm_rows_kernel(Mxfp4G
 // With one wave per SIMD every instruction takes an issue slot of ~5 cycles and an MFMA 16, so the side work goes between single MFMAs ("slots"),
 // about one instruction at a time (measured: what an instruction costs beyond that is 4 cycles each).
 // A lane's four scale bytes of a group (one per step) are one register, the byte is chosen by the MFMA's op_sel.
-// Measured: 4608 x 36864 x 4096 354 us = 3.9 PF, 4608 x 16384 x 16384 529 us = 4.7 PF.  Bound by the matrix pipe's power and by the delivery L2 -> LDS
+// Measured: 4608 x 36864 x 4096 351 us = 4.0 PF, 4608 x 16384 x 16384 529 us = 4.7 PF.  Bound by the matrix pipe's power and by the delivery L2 -> LDS
 // together: a group takes 3.5 us, without its requests 2.5, without its LDS reads 3.4, without either 2.4 (7.3 PF, the clock down to 1.8 GHz; the same
 // loop on zero operands: 2.8, 1.9 without requests).  A tile's prologue and its output take 8 us.
 // Steps behind K: addresses stay inside the row and both scale bytes are 0, 2^-254 times finite codes, which is below f32: exactly 0.
@@ -568,7 +568,8 @@ __global__ __launch_bounds__(256, PER_CU) void mxfp4_gemm_tile_kernel(Mxfp4Gemm 
 // BM x BN outputs per workgroup of KG WM x WN waves: group kg of the waves takes the 128-k steps KG t + kg, and the groups' sums are added through LDS at
 // the end.  With few tiles a CU holds one, and a stage of it takes ~1200 cycles whatever its size (wait, barrier, LDS reads, MFMAs, requests: one wave per
 // SIMD issues them in turn), so what counts is how many k a stage holds: 64 x 4096 x 4096 with 64 x 64 tiles and two groups 11.3 us, four 9.4, four and 32 x 64
-// tiles 7.4 (the 128 x 128 tiles above 11.9).  Bound by that latency: 16 x 36864 x 4096 17.6 us = 4.6 TB/s of W, 16 x 12288 x 4096 7.2.  A stage is KG / 2 pairs of steps, a pair 128 bytes of every row (pieces and swizzle as above), in a ring of STAGES buffers,
+// tiles 7.4 (the 128 x 128 tiles above 11.9).  Bound by that latency: 16 x 36864 x 4096 17.6 us = 4.6 TB/s of W, 16 x 12288 x 4096 7.2
+// (W from HBM: 19.3, 8.2).  A stage is KG / 2 pairs of steps, a pair 128 bytes of every row (pieces and swizzle as above), in a ring of STAGES buffers,
 // STAGES - 1 of them requested ahead with a counted wait.  The scales of 16 steps come at once, one dword per row and step, ahead of the first of them;
 // slot c of a row holds step c ^ (row / 4) % 4 of the 16, so that the 16 rows a fragment reads lie in different banks.
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool BF16, bool VEC>
@@ -688,7 +689,7 @@ bool wide_rows(const Mxfp4Gemm& p) {
 // A is shared by every wave of a workgroup and comes once per workgroup through LDS, `chunk` steps of all its rows at a time (a multiple of the waves' U steps, so
 // that a wave's steps wave, wave + WAVES, ... fall into the chunks alike); W and its scales stream through registers across the chunks.
 // Read by every wave for itself, A costs four loads per step against one of W: the vector-memory path, not HBM, is then the bound.
-// Measured: 1 x 19456 x 2560 8.6 us = 3.1 TB/s of W; bound by the latency of staging A and of a wave's first loads.
+// Measured: 1 x 19456 x 2560 9.3 us = 2.8 TB/s of W from HBM; bound by the latency of staging A and of a wave's first loads.
 constexpr int BF16_ROWS_U = 2, BF16_ROWS_WAVES = 8;
 template <bool AVEC, bool VEC>
 __global__ __launch_bounds__(64 * BF16_ROWS_WAVES) void bf16_mxfp4_gemm_rows_kernel(Mxfp4Gemm p, int tiles_n, int chunk) {
@@ -757,9 +758,12 @@ __global__ __launch_bounds__(64 * BF16_ROWS_WAVES) void bf16_mxfp4_gemm_rows_ker
 // W's codes become bf16 in registers (4 conversions per 8 values, used by MT MFMAs), a lane's scale is one byte of the row's four.
 // Chunks of 16 bytes are swizzled (A: within each 128-byte half by row & 7; W: the same where the codes of two steps come as one 128-byte line, else
 // the 64 bytes by (row / 2) & 3) so that fragment reads meet no bank conflicts.
-// Measured: 23 x 5120 x 5120 9.1 us, 512 x 4096 x 12288 53 us = 0.97 PF, 4608 x 12288 x 4096 370 us = 1.25 PF; bound by the conversions, which share the
-// issue slots with the MFMAs, and with few rows by the latency of a stage.
-// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead (512 x 4096 x 4095: 40 us, x 4096 21).  Columns >= K are zeroed where
+// Measured (W from HBM): 23 x 5121 x 5120 11.9 us, 512 x 4096 x 12288 57 us = 0.90 PF (53 with W in the 256 MB cache), 4608 x 12288 x 4096 370 us =
+// 1.25 PF.  With few rows bound by the latency of a stage.  What the larger ones spend, us at 512 x 4096 x 12288 / 4608 x 12288 x 4096 in one run: all 58 / 393,
+// without the requests 46 / 319, without A's LDS reads 54 / 367, without the conversions 56 / 389, without A's reads and the conversions 51 / 347, without any
+// of the three 39 / 286: first the delivery into LDS, then A's fragments, which every wave of a k group reads for itself (72 KB of LDS reads per 128 k of a
+// 64 x 128 tile, 576 clocks beside 512 of MFMAs), the conversions last.
+// A by DMA needs rows of whole dwords (AVEC: even K and row stride); other rows pass through registers, a stage ahead (512 x 4096 x 4095: 38 to 46 us, x 4096 21).  Columns >= K are zeroed where
 // the last stage is read or staged.
 __device__ __forceinline__ bf16x8 zero_from(bf16x8 v, int keep) {   // values [keep, 8) become zero
     u32x4 u = __builtin_bit_cast(u32x4, v);

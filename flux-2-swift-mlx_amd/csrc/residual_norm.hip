@@ -5,7 +5,8 @@
 //   out  = norm(x') * w * (1 + scale) + shift    the next block's operand
 // gate, scale and shift are per column, one set for rows < split (text) and one for the others (image), as in layernorm_modulate.
 //
-// Measured: 4608 x 4096 (y, out bf16) 53 us = 4.3 TB/s, 1031 x 5119 f32 22 us = 3.8 TB/s, one row of 2560 4.2 us (a launch and two sums).
+// Measured: 4608 x 4096 (y, out bf16) 52 us = 4.4 TB/s, 1031 x 5119 f32 23 us = 3.6 TB/s, with y and out in bf16 27 us = 2.3 TB/s (odd rows go value by
+// value), 4608 x 12000 191 us, one row of 2560 4.2 us (a launch and two sums).
 // Bound by HBM: x and y are read once, x' and out written once; a row lives in the registers of the threads that own it, its statistics
 // are f32 sums over those registers (the variance around the mean of the row, in a second sum over registers, not E[x^2] - mean^2).  What hides
 // the sums' and the vectors' latency is other rows' workgroups, so few registers count for more than early loads or vectors kept over several rows (both
